@@ -564,6 +564,80 @@ KM_API int km_node_product_f32(int64_t k, int64_t n, int64_t nodes_per_block, in
 
 
 /* ---------------------------------------------------------------------------------------
+ * Sequence operators.  No reference counterpart: like the products above they apply matrices that are
+ * generated on the fly, here over the tokens of sequences.
+ *
+ * Element types (`KM_TYPE_*`) are given per call; state, decays, norms and gradients of decays are fp32.
+ * Strides are in elements, int64.
+ * ------------------------------------------------------------------------------------- */
+#define KM_TYPE_F32 0
+#define KM_TYPE_BF16 1
+#define KM_TYPE_F16 2
+#define KM_TYPE_I32 3
+#define KM_TYPE_I64 4
+#define KM_TYPE_F64 5
+
+/* Rotary positions.  For i < pairs, with (a, b) the i-th pair of a head's values and w = position * frequency[i]
+ * (in 64 bits, as are the angle's reduction and the frequencies):
+ *   (a, b) -> scale (a cos w - sign b sin w, sign a sin w + b cos w),  sign = inverse ? -1 : 1
+ * the pairs being (i, i + pairs) or, interleaved, (2 i, 2 i + 1); values from 2 pairs on are copied.
+ * Up to two operands (q and k) with the same positions: views with batch_stride[0] = batch, batch_stride[1] = head,
+ * stride[0] = token, stride[1] = value; `heads[1] = 0` for one operand.  positions: batch_stride[0] and stride[0], of
+ * type int32, int64 or fp32. */
+KM_API int km_rotary(int32_t dtype, int64_t batch, int64_t tokens, const int64_t heads[2], int64_t dim, int64_t pairs,
+                     const km_view in[2], const km_view out[2], int32_t position_type, const km_view *positions,
+                     int32_t frequency_type, const void *frequencies, int32_t interleaved, int32_t inverse, float scale, void *stream);
+
+/* Linear attention with a decay for each head.  With the state S (dk x dv) of a (sequence, head),
+ *   S_t = e^g S_{t-1} + k_t v_t^T,   out_t = scale S_t^T q_t,   g = log_decay[head],
+ * i.e. the product of the matrix e^{g (t - s)} (q_t . k_s), s <= t, which is generated on the fly, with v.
+ *
+ * `reverse`: the same backwards in time, in the form of a gradient: with W_t = scale k_t v_t^T + e^g W_{t+1},
+ * where e^g W_{len} is state_in as it is, out_t = W_t^T q_t, and state_out = e^g W_0.  With (q, k, v, state_in):
+ *   dq = forward (dout, v, k, S_0^T),  dk = reverse (v, dout, q, dS^T),  dv and dS_0 = reverse (k, q, dout, dS).
+ *
+ * Sequences are batches of `tokens` rows, or, with `starts` (sequences + 1 device int32 that do not decrease),
+ * the rows [starts[i], starts[i + 1]) of one batch of `tokens` rows; rows of no sequence get zeros.  (starts are
+ * clamped to [0, tokens].)  Operand views: batch_stride[0] = sequence, batch_stride[1] = group of heads, batch_stride[2] =
+ * head inside the group (0: the group shares the operand), stride[0] = token, stride[1] = value.  State views: the same
+ * batch strides, stride[0] = dk, stride[1] = dv; state_in null: zeros; state_out null: not wanted.
+ *
+ * path: 0 automatic, 1 FMA pipe (any type), 2 tensor cores (16-bit types).  dk and dv: 1 to KM_DECAY_MAX_DIM. */
+#define KM_DECAY_MAX_DIM 128
+typedef struct km_decay_problem {
+    int32_t dtype, out_dtype; /* out_dtype: dtype or KM_TYPE_F32 */
+    int32_t reverse, path;
+    int64_t sequences, tokens, groups, group, dk, dv;
+    int32_t packed;
+    float scale;
+} km_decay_problem;
+KM_API size_t km_decay_attention_workspace_bytes(const km_decay_problem *problem);
+KM_API int km_decay_attention(const km_decay_problem *problem, const km_view *q, const km_view *k, const km_view *v, const km_view *out,
+                              const float *log_decay, const int32_t *starts, const km_view *state_in, const km_view *state_out,
+                              void *workspace, size_t workspace_bytes, void *stream);
+/* grad[head] = d loss / d log_decay[head] for the forward form, from dout = d loss / d out and dstate = d loss / d state_out
+ * (null: none).  Deterministic. */
+KM_API size_t km_decay_gradient_workspace_bytes(const km_decay_problem *problem);
+KM_API int km_decay_gradient(const km_decay_problem *problem, const km_view *q, const km_view *k, const km_view *v, const km_view *dout,
+                             const float *log_decay, const int32_t *starts, const km_view *state_in, const km_view *dstate,
+                             float *grad, void *workspace, size_t workspace_bytes, void *stream);
+/* out (rows, groups, dim) = the sums over each group of in (rows, groups, group, dim), fp32, both contiguous; out of type dtype. */
+KM_API int km_group_sums(int32_t dtype, int64_t rows, int64_t groups, int64_t group, int64_t dim, const float *in, void *out, void *stream);
+/* One token for each row: the recurrence once, in place on states[slot of the row] (null slots: the row itself).
+ * A row whose slot is not in [0, pool) gets zeros and touches no state; rows with the same slot are tokens of one sequence,
+ * in their order.  Views of q, k, v, out: batch_stride[0] = row, [1] = group, [2] = head inside it, stride[1] = 1 = value;
+ * states: batch_stride[0] = slot, [1], [2], stride[0] = dk, stride[1] = 1. */
+KM_API int km_decay_step(int32_t dtype, int64_t rows, int64_t pool, int64_t groups, int64_t group, int64_t dk, int64_t dv,
+                         const km_view *q, const km_view *k, const km_view *v, const km_view *out, const float *log_decay,
+                         const km_view *states, int32_t slot_type, const void *slots, float scale, void *stream);
+
+/* The 2-norm of all elements of `count` tensors (contiguous, of the types given), and, with scale_in_place, the tensors times
+ * min(1, max_norm / (norm + eps)) where that is below one (or not a number).  *norm is fp32.  The tensors may not overlap.  Deterministic. */
+KM_API size_t km_global_norm_workspace_bytes(int64_t count);
+KM_API int km_global_norm(int64_t count, void *const *tensors, const int64_t *elements, const int32_t *types, int32_t scale_in_place,
+                          double max_norm, double eps, float *norm, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
  * Self-tests of the give-up path of the tensor-core kernels.  No reference counterpart (the
  * reference's debug build synchronises and throws on a CUDA error,
  * native/common/gpu_assert.cuh:6-23; its kernels have no hand-offs that could stall).

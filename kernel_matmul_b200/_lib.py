@@ -30,6 +30,14 @@ class KmView(ctypes.Structure):
     ]
 
 
+class KmDecayProblem(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("reverse", ctypes.c_int32), ("path", ctypes.c_int32),
+        ("sequences", ctypes.c_int64), ("tokens", ctypes.c_int64), ("groups", ctypes.c_int64), ("group", ctypes.c_int64),
+        ("dk", ctypes.c_int64), ("dv", ctypes.c_int64), ("packed", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
 class KmError(RuntimeError):
     """An entry point of libkm_b200 returned a non-zero status."""
 
@@ -153,6 +161,25 @@ def _load() -> ctypes.CDLL:
     lib.km_node_update_p_f32.argtypes = [i64, i64, i64, vp, vp, vp, vp, i64, i64, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp]
     lib.km_node_product_f32.restype = ctypes.c_int
     lib.km_node_product_f32.argtypes = [i64, i64, i64, i64, ip, ip, vp, vp, vp, i64, i64, vp, vp, f32, vp, vp]
+    dp, ip64 = ctypes.POINTER(KmDecayProblem), ctypes.POINTER(i64)
+    lib.km_rotary.restype = ctypes.c_int
+    lib.km_rotary.argtypes = [i32, i64, i64, ip64, i64, i64, wp, wp, i32, wp, i32, vp, i32, i32, f32, vp]
+    lib.km_decay_attention_workspace_bytes.restype = sz
+    lib.km_decay_attention_workspace_bytes.argtypes = [dp]
+    lib.km_decay_attention.restype = ctypes.c_int
+    lib.km_decay_attention.argtypes = [dp, wp, wp, wp, wp, vp, vp, wp, wp, vp, sz, vp]
+    lib.km_decay_gradient_workspace_bytes.restype = sz
+    lib.km_decay_gradient_workspace_bytes.argtypes = [dp]
+    lib.km_decay_gradient.restype = ctypes.c_int
+    lib.km_decay_gradient.argtypes = [dp, wp, wp, wp, wp, vp, vp, wp, wp, vp, vp, sz, vp]
+    lib.km_group_sums.restype = ctypes.c_int
+    lib.km_group_sums.argtypes = [i32, i64, i64, i64, i64, vp, vp, vp]
+    lib.km_decay_step.restype = ctypes.c_int
+    lib.km_decay_step.argtypes = [i32, i64, i64, i64, i64, i64, i64, wp, wp, wp, wp, vp, wp, i32, vp, f32, vp]
+    lib.km_global_norm_workspace_bytes.restype = sz
+    lib.km_global_norm_workspace_bytes.argtypes = [i64]
+    lib.km_global_norm.restype = ctypes.c_int
+    lib.km_global_norm.argtypes = [i64, pp, ip64, ctypes.POINTER(i32), i32, ctypes.c_double, ctypes.c_double, vp, vp, sz, vp]
     lib.km_selftest_bounded_wait.restype = ctypes.c_int
     lib.km_selftest_bounded_wait.argtypes = [i64, vp, vp]
     lib.km_selftest_set_wait_polls.restype = ctypes.c_int
@@ -174,6 +201,8 @@ EXPORTED = [
     "km_cg_block_dots_f32", "km_cg_q_dots_f32", "km_cg_segment_sums_f32", "km_cg_init_scalars_f32", "km_cg_update_xr_f32",
     "km_cg_update_p_f32", "km_cg_log_forms_f32", "km_node_operator_plan_f32", "km_node_operator_build_f32", "km_node_operator_changed", "km_node_compress_f32", "km_node_update_p_f32",
     "km_node_product_f32", "km_sum_phases_workspace_bytes", "km_sum_phases_prepare_f32", "km_matmul_rows_phases_f32",
+    "km_rotary", "km_decay_attention_workspace_bytes", "km_decay_attention", "km_decay_gradient_workspace_bytes", "km_decay_gradient",
+    "km_group_sums", "km_decay_step", "km_global_norm_workspace_bytes", "km_global_norm",
 ]
 
 

@@ -1,0 +1,748 @@
+// Linear attention with a decay for each head (km_decay.cuh has the method): the kernels on the FMA pipe, the scan
+// over a sequence's segments, the gradient of the decays, sums over groups of heads and the recurrence for single tokens;
+// the entry points for all of them.
+#include "km_decay.cuh"
+
+namespace km {
+
+// ------------------------------------------------------------------------------------------------
+// Whole sequences on the FMA pipe: fp32 operands (products of fp32 values have no exact form on the tensor cores), and the
+// other types on path 1.  One CTA of 256 threads per (segment, head); chunks of 32 tokens, so that the products inside a
+// chunk (32 x 32 x (dk + dv)) cost a quarter of those with the state (2 x 32 x dk x dv).  The state is held in registers,
+// 8 x 8 values per thread, for its update, and in shared memory for the product with q.
+constexpr int FC = 32;          // tokens of a chunk
+constexpr int FLD = 132;        // floats of a row of q, k, v in shared memory
+constexpr int FMA_SMEM = (3 * FC * FLD + FC * 36 + KM_DECAY_MAX_DIM * KM_DECAY_MAX_DIM) * 4;
+
+template <typename T>
+__device__ __forceinline__ void load_chunk(float *dst, const DecayArgs &a, const Segment &s, const Operand &o, int64_t hg, int64_t hi,
+                                           int64_t first, int tokens, int dim, int ld, int width) {
+    const T *src = o.at<T>(a.starts == nullptr ? s.seq : 0, hg, hi);
+    for (int i = threadIdx.x; i < FC * width; i += blockDim.x) {
+        const int t = i / width, c = i - t * width;
+        float x = 0.0f;
+        if (t < tokens && c < dim) x = as_float(src[token_row(a, s, first + t) * o.row + c * o.col]);
+        dst[t * ld + c] = x;
+    }
+}
+
+template <typename T, typename O, bool STATE_ONLY>
+__global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    float *sq = smem, *sk = sq + FC * FLD, *sv = sk + FC * FLD, *sp = sv + FC * FLD, *sz = sp + FC * 36;
+    const int64_t h = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
+    const int64_t hg = h / a.group, hi = h - hg * a.group;
+    const Segment s = find_segment(a, slot);
+    if (!STATE_ONLY && s.spare >= 0) clear_spare_rows<O>(a, s, hg, hi);
+    if (!s.used || (STATE_ONLY && s.last)) return;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const float g2 = log2_decay(a.log_decay[h]);
+    const int dk4 = (a.dk + 3) & ~3;
+
+    // state: rows ty + 16 i, columns 4 tx + 64 j .. + 3
+    float z[8][8];
+    const bool first_segment = s.first == 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
+            float x = 0.0f;
+            if (!STATE_ONLY && r < a.dk && c < a.dv) {
+                if (!first_segment)
+                    x = a.states[((slot * a.heads + h) * a.dk + r) * a.dv + c];
+                else if (a.state_in.data != nullptr)
+                    x = a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + c * a.state_in.col];
+            }
+            z[i][j] = x;
+        }
+    if (!STATE_ONLY && s.length == 0) {  // nothing to go through: the state as it came
+        if (a.state_out.data != nullptr)
+            for (int i = 0; i < 8; i++)
+                for (int j = 0; j < 8; j++) {
+                    const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
+                    if (r < a.dk && c < a.dv) a.state_out.at<float>(s.seq, hg, hi)[r * a.state_out.row + c * a.state_out.col] = z[i][j];
+                }
+        return;
+    }
+    if (!STATE_ONLY && first_segment && !a.reverse) {
+        const float w = exp2f(g2);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) z[i][j] *= w;
+    }
+
+    for (int64_t first = s.first; first < s.first + s.count; first += FC) {
+        const int tokens = (int)min((int64_t)FC, s.first + s.count - first);
+        const bool final = first + tokens == s.length;
+        const int e = final && !a.reverse ? tokens - 1 : tokens;
+        __syncthreads();
+        if (!STATE_ONLY) load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
+        load_chunk<T>(sk, a, s, a.k, hg, hi, first, tokens, a.dk, FLD, 128);
+        load_chunk<T>(sv, a, s, a.v, hg, hi, first, tokens, a.dv, FLD, 128);
+        if (!STATE_ONLY) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    *reinterpret_cast<float4 *>(sz + (ty + 16 * i) * 128 + 4 * tx + 64 * j) =
+                        make_float4(z[i][4 * j], z[i][4 * j + 1], z[i][4 * j + 2], z[i][4 * j + 3]);
+        }
+        __syncthreads();
+        if (!STATE_ONLY) {
+            float p[2][2] = {};
+            for (int c = 0; c < dk4; c += 4) {
+                float4 x[2], y[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    x[i] = *reinterpret_cast<const float4 *>(sq + (ty + 16 * i) * FLD + c);
+                    y[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * FLD + c);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        p[i][j] = fmaf(x[i].x, y[j].x, p[i][j]);
+                        p[i][j] = fmaf(x[i].y, y[j].y, p[i][j]);
+                        p[i][j] = fmaf(x[i].z, y[j].z, p[i][j]);
+                        p[i][j] = fmaf(x[i].w, y[j].w, p[i][j]);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int t = ty + 16 * i, u = tx + 16 * j;
+                    sp[t * 36 + u] = t >= u ? p[i][j] * exp2f(g2 * (float)(t - u)) * (a.scale_in * a.scale_out) : 0.0f;
+                }
+            __syncthreads();
+            float o[2][8] = {};
+            for (int c = 0; c < a.dk; c++) {
+                const float4 z0 = *reinterpret_cast<const float4 *>(sz + c * 128 + 4 * tx);
+                const float4 z1 = *reinterpret_cast<const float4 *>(sz + c * 128 + 4 * tx + 64);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float x = sq[(ty + 16 * i) * FLD + c];
+                    o[i][0] = fmaf(x, z0.x, o[i][0]), o[i][1] = fmaf(x, z0.y, o[i][1]);
+                    o[i][2] = fmaf(x, z0.z, o[i][2]), o[i][3] = fmaf(x, z0.w, o[i][3]);
+                    o[i][4] = fmaf(x, z1.x, o[i][4]), o[i][5] = fmaf(x, z1.y, o[i][5]);
+                    o[i][6] = fmaf(x, z1.z, o[i][6]), o[i][7] = fmaf(x, z1.w, o[i][7]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float w = exp2f(g2 * (float)(ty + 16 * i)) * a.scale_out;
+#pragma unroll
+                for (int j = 0; j < 8; j++) o[i][j] *= w;
+            }
+            for (int u = 0; u < tokens; u++) {
+                const float4 v0 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx);
+                const float4 v1 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx + 64);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float x = sp[(ty + 16 * i) * 36 + u];
+                    if (u > ty + 16 * i) continue;  // later tokens do not reach this one, not even as 0 * inf
+                    o[i][0] = fmaf(x, v0.x, o[i][0]), o[i][1] = fmaf(x, v0.y, o[i][1]);
+                    o[i][2] = fmaf(x, v0.z, o[i][2]), o[i][3] = fmaf(x, v0.w, o[i][3]);
+                    o[i][4] = fmaf(x, v1.x, o[i][4]), o[i][5] = fmaf(x, v1.y, o[i][5]);
+                    o[i][6] = fmaf(x, v1.z, o[i][6]), o[i][7] = fmaf(x, v1.w, o[i][7]);
+                }
+            }
+            O *out = a.out.at<O>(a.starts == nullptr ? s.seq : 0, hg, hi);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int t = ty + 16 * i;
+                if (t >= tokens) continue;
+                O *row = out + token_row(a, s, first + t) * a.out.row;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int c = 4 * tx + 64 * (j >> 2) + (j & 3);
+                    if (c < a.dv) row[c * a.out.col] = from_float<O>(o[i][j]);
+                }
+            }
+        }
+        const float carry = exp2f(g2 * (float)e);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) z[i][j] *= carry;
+        for (int u = 0; u < tokens; u++) {
+            const float w = exp2f(g2 * (float)(e - u)) * a.scale_in;
+            const float4 v0 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx);
+            const float4 v1 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx + 64);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x = sk[u * FLD + ty + 16 * i] * w;
+                z[i][0] = fmaf(x, v0.x, z[i][0]), z[i][1] = fmaf(x, v0.y, z[i][1]);
+                z[i][2] = fmaf(x, v0.z, z[i][2]), z[i][3] = fmaf(x, v0.w, z[i][3]);
+                z[i][4] = fmaf(x, v1.x, z[i][4]), z[i][5] = fmaf(x, v1.y, z[i][5]);
+                z[i][6] = fmaf(x, v1.z, z[i][6]), z[i][7] = fmaf(x, v1.w, z[i][7]);
+            }
+        }
+    }
+    if (STATE_ONLY || (s.last && a.state_out.data != nullptr)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
+                if (r >= a.dk || c >= a.dv) continue;
+                if (STATE_ONLY)
+                    a.states[((slot * a.heads + h) * a.dk + r) * a.dv + c] = z[i][j];
+                else
+                    a.state_out.at<float>(s.seq, hg, hi)[r * a.state_out.row + c * a.state_out.col] = z[i][j];
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// States at the start of each segment, in place: states[slot] held the segment's own contribution.  The segments of a
+// sequence one after the other, its values spread over 8 x 256 threads: each value is read and written once.
+__global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
+    const int64_t h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
+    const int64_t hg = h / a.group, hi = h - hg * a.group;
+    const int64_t slot0 = segments_before(a, seq);
+    int64_t begin, length;
+    sequence_rows(a, seq, begin, length);
+    const int64_t n = min(segments_of(a, length), a.slots - slot0);
+    if (n <= 1) return;
+    const float g2 = log2_decay(a.log_decay[h]);
+    const float carry = exp2f(g2 * (float)a.segment), enter = a.reverse ? 1.0f : exp2f(g2);
+    const int values = a.dk * a.dv;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < values; i += 256 * gridDim.y) {
+        float zv = 0.0f;
+        if (a.state_in.data != nullptr)
+            zv = enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col];
+        float *p = a.states + (slot0 * a.heads + h) * (int64_t)values + i;
+        const int64_t step = a.heads * (int64_t)values;
+        float own = *p;
+        for (int64_t j = 1; j < n; j++) {
+            p += step;
+            zv = fmaf(carry, zv, own);
+            own = j + 1 < n ? *p : 0.0f;
+            *p = zv;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Gradient of the log decays.  With M = dZ/dg the chunk's outputs change with g by
+//   d out_t = scale [ sum_s (t - s) e^{g (t - s)} (q_t . k_s) v_s + e^{g t} (t Z + M)^T q_t ],
+//   M <- e^{g e} (e Z + M) + sum_s (e - s) e^{g (e - s)} k_s v_s^T,
+// and grad = sum_t dout_t . d out_t + <dstate, dM of the last state>: a sum of terms that are each as small as their
+// distances, where differences of sums over tokens (t q.dq - s k.dk) would cancel to a part of 1 / tokens.
+// One CTA per (sequence, head, 32 columns of v): the states' columns are independent.  All in fp32, sums over chunks in fp64.
+constexpr int GV = 32;  // columns of v
+constexpr int GRAD_SMEM = (2 * FC * FLD + 2 * FC * 36 + FC * 36 + 2 * KM_DECAY_MAX_DIM * 36) * 4;
+
+template <typename T>
+__global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operand dout, Operand dstate, int vblocks, double *partials) {
+    extern __shared__ __align__(16) float smem[];
+    float *sq = smem, *sk = sq + FC * FLD, *sv = sk + FC * FLD, *sd = sv + FC * 36, *sp = sd + FC * 36, *sz = sp + FC * 36,
+          *sm = sz + KM_DECAY_MAX_DIM * 36;
+    const int vb = blockIdx.x % vblocks;
+    const int64_t rest = blockIdx.x / vblocks, h = rest % a.heads, seq = rest / a.heads;
+    const int64_t hg = h / a.group, hi = h - hg * a.group;
+    Segment s = {};
+    s.seq = seq;
+    sequence_rows(a, seq, s.begin, s.length);
+    const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;  // columns 4 tx .. + 3, rows ty + 32 i
+    const int cols = min(GV, a.dv - vb * GV), dk4 = (a.dk + 3) & ~3;
+    const float g2 = log2_decay(a.log_decay[h]);
+    Operand v = a.v, d = dout;
+    v.data += vb * GV * v.col * (int64_t)sizeof(T);
+    d.data += vb * GV * d.col * (int64_t)sizeof(T);
+    float z[4][4], m[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int r = ty + 32 * i, c = 4 * tx + j;
+            float x = 0.0f;
+            if (a.state_in.data != nullptr && r < a.dk && c < cols)
+                x = exp2f(g2) * a.state_in.at<float>(seq, hg, hi)[r * a.state_in.row + (vb * GV + c) * a.state_in.col];
+            z[i][j] = m[i][j] = x;
+        }
+    double total = 0.0;
+    for (int64_t first = 0; first < s.length; first += FC) {
+        const int tokens = (int)min((int64_t)FC, s.length - first);
+        const int e = first + tokens == s.length ? tokens - 1 : tokens;
+        __syncthreads();
+        load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
+        load_chunk<T>(sk, a, s, a.k, hg, hi, first, tokens, a.dk, FLD, 128);
+        load_chunk<T>(sv, a, s, v, hg, hi, first, tokens, cols, 36, GV);
+        load_chunk<T>(sd, a, s, d, hg, hi, first, tokens, cols, 36, GV);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            *reinterpret_cast<float4 *>(sz + (ty + 32 * i) * 36 + 4 * tx) = make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
+            *reinterpret_cast<float4 *>(sm + (ty + 32 * i) * 36 + 4 * tx) = make_float4(m[i][0], m[i][1], m[i][2], m[i][3]);
+        }
+        __syncthreads();
+        float sum = 0.0f;
+        {  // inside the chunk: entries (t, u) with t = ty, u = tx + 8 i
+            float p[4] = {}, r[4] = {};
+            for (int c = 0; c < dk4; c += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(sq + ty * FLD + c);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(sk + (tx + 8 * i) * FLD + c);
+                    p[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, p[i]))));
+                }
+            }
+            for (int c = 0; c < GV; c += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(sd + ty * 36 + c);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(sv + (tx + 8 * i) * 36 + c);
+                    r[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, r[i]))));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int u = tx + 8 * i;
+                if (ty > u) sum = fmaf((float)(ty - u) * exp2f(g2 * (float)(ty - u)) * p[i], r[i], sum);
+            }
+        }
+        {  // from the states: row t = ty, columns 4 tx ..
+            float x[4] = {}, y[4] = {};
+            for (int c = 0; c < a.dk; c++) {
+                const float qv = sq[ty * FLD + c];
+                const float4 zz = *reinterpret_cast<const float4 *>(sz + c * 36 + 4 * tx);
+                const float4 mm = *reinterpret_cast<const float4 *>(sm + c * 36 + 4 * tx);
+                x[0] = fmaf(qv, zz.x, x[0]), x[1] = fmaf(qv, zz.y, x[1]), x[2] = fmaf(qv, zz.z, x[2]), x[3] = fmaf(qv, zz.w, x[3]);
+                y[0] = fmaf(qv, mm.x, y[0]), y[1] = fmaf(qv, mm.y, y[1]), y[2] = fmaf(qv, mm.z, y[2]), y[3] = fmaf(qv, mm.w, y[3]);
+            }
+            const float w = exp2f(g2 * (float)ty);
+            float part = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) part = fmaf(fmaf((float)ty, x[j], y[j]), sd[ty * 36 + 4 * tx + j], part);
+            if (ty < tokens) sum = fmaf(w, part, sum);
+        }
+        total += (double)sum * (double)a.scale_out;
+        const float carry = exp2f(g2 * (float)e);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                m[i][j] = carry * fmaf((float)e, z[i][j], m[i][j]);
+                z[i][j] *= carry;
+            }
+        for (int u = 0; u < tokens; u++) {
+            const float w = exp2f(g2 * (float)(e - u)), wm = w * (float)(e - u);
+            const float4 vv = *reinterpret_cast<const float4 *>(sv + u * 36 + 4 * tx);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float kk = sk[u * FLD + ty + 32 * i], x = kk * w, y = kk * wm;
+                z[i][0] = fmaf(x, vv.x, z[i][0]), z[i][1] = fmaf(x, vv.y, z[i][1]), z[i][2] = fmaf(x, vv.z, z[i][2]),
+                z[i][3] = fmaf(x, vv.w, z[i][3]);
+                m[i][0] = fmaf(y, vv.x, m[i][0]), m[i][1] = fmaf(y, vv.y, m[i][1]), m[i][2] = fmaf(y, vv.z, m[i][2]),
+                m[i][3] = fmaf(y, vv.w, m[i][3]);
+            }
+        }
+    }
+    if (dstate.data != nullptr && s.length > 0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = ty + 32 * i, c = 4 * tx + j;
+                // (m holds e^{g e} (e Z + M) + ..: the derivative of the last state, whose Z is e^g S_0 with M = Z)
+                if (r < a.dk && c < cols)
+                    total += (double)m[i][j] * (double)dstate.at<float>(seq, hg, hi)[r * dstate.row + (vb * GV + c) * dstate.col];
+            }
+    }
+    __shared__ double warp_sum[8];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if ((tid & 31) == 0) warp_sum[tid >> 5] = total;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < 8; w++) total += warp_sum[w];
+        partials[(h * a.sequences + seq) * vblocks + vb] = total;
+    }
+}
+
+__global__ void __launch_bounds__(256) decay_gradient_finish_kernel(int64_t count, const double *partials, float *grad) {
+    __shared__ double warp_sum[8];
+    const int64_t h = blockIdx.x;
+    double v = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += 256) v += partials[h * count + i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; w++) v += warp_sum[w];
+        grad[h] = (float)v;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) group_sums_kernel(int64_t count, int64_t group, int64_t dim, const float *in, T *out) {
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < count; i += 256LL * gridDim.x) {
+        const int64_t rg = i / dim, c = i - rg * dim;
+        const float *p = in + rg * group * dim + c;
+        float v = 0.0f;
+        for (int64_t j = 0; j < group; j++) v += p[j * dim];
+        out[i] = from_float<T>(v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// One token: S <- e^g S + k v^T, out = scale S^T q.  Reading and writing the state is all the time there is.  A CTA of
+// 256 threads per (row, head, COLS columns of v): a thread holds VEC neighbouring columns of every (256 VEC / COLS)-th
+// row of the state, all of them loaded before the first is used; the sums over dk go through shared memory.
+template <typename T, int VEC, int COLS>
+__global__ void __launch_bounds__(256, COLS == 128 ? 2 : 4) decay_step_kernel(int64_t rows, int64_t pool, int64_t heads, int64_t group, int dk, int dv, Operand q,
+                                                         Operand k, Operand v, Operand out, const float *log_decay, Operand states,
+                                                         int slot_type, const void *slots, float scale) {
+    constexpr int TX = COLS / VEC, TY = 256 / TX, N = (KM_DECAY_MAX_DIM + TY - 1) / TY;
+    __shared__ float part[TY][COLS + 4];
+    __shared__ float sq[KM_DECAY_MAX_DIM], sk[KM_DECAY_MAX_DIM];
+    const int vblocks = (dv + COLS - 1) / COLS;
+    const int vb = blockIdx.x % vblocks;
+    const int64_t rest = blockIdx.x / vblocks, h = rest % heads;
+    int64_t row = rest / heads;
+    const int64_t hg = h / group, hi = h - hg * group;
+    const int tid = threadIdx.x, tx = tid % TX, ty = tid / TX, col = vb * COLS + tx * VEC;
+    const auto slot_of = [&](int64_t r) -> int64_t {
+        if (slots == nullptr) return r;
+        return slot_type == KM_TYPE_I32 ? static_cast<const int32_t *>(slots)[r] : static_cast<const int64_t *>(slots)[r];
+    };
+    const int64_t slot = slot_of(row);
+    const bool valid = slot >= 0 && slot < pool;
+    // rows with the same slot: the first one's CTA takes them all, in order
+    bool again = false;
+    if (slots != nullptr && valid) {
+        bool earlier = false, later = false;
+        for (int64_t r = tid; r < rows; r += 256) {
+            const bool same = slot_of(r) == slot;
+            earlier = earlier || (same && r < row);
+            later = later || (same && r > row);
+        }
+        if (__syncthreads_or(earlier)) return;
+        again = __syncthreads_or(later);
+    }
+    const bool mine = col < dv;
+    if (!valid) {
+        if (mine && ty == 0)
+            for (int j = 0; j < VEC; j++)
+                if (col + j < dv) out.at<T>(row, hg, hi)[col + j] = from_float<T>(0.0f);
+        return;
+    }
+    const float decay = exp2f(log2_decay(log_decay[h]));
+    float *state = states.at<float>(slot, hg, hi) + col;
+    float s[N][VEC];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int r = ty + i * TY;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) s[i][j] = 0.0f;
+        if (mine && r < dk) {
+            if constexpr (VEC == 4) {
+                const float4 x = __ldcs(reinterpret_cast<const float4 *>(state + r * states.row));
+                s[i][0] = x.x, s[i][1] = x.y, s[i][2] = x.z, s[i][3] = x.w;
+            } else {
+                s[i][0] = state[r * states.row];
+            }
+        }
+    }
+    for (;;) {
+        for (int c = tid; c < dk; c += 256) {
+            sq[c] = as_float(q.at<const T>(row, hg, hi)[c]);
+            sk[c] = as_float(k.at<const T>(row, hg, hi)[c]);
+        }
+        float vv[VEC], o[VEC] = {};
+#pragma unroll
+        for (int j = 0; j < VEC; j++) vv[j] = col + j < dv ? as_float(v.at<const T>(row, hg, hi)[col + j]) : 0.0f;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int r = ty + i * TY;
+            if (r < dk) {
+                const float kk = sk[r], qq = sq[r];
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    s[i][j] = fmaf(decay, s[i][j], kk * vv[j]);
+                    o[j] = fmaf(qq, s[i][j], o[j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; j++) part[ty][tx * VEC + j] = o[j];
+        __syncthreads();
+        for (int c = tid; c < COLS; c += 256) {
+            if (vb * COLS + c >= dv) continue;
+            float sum = 0.0f;
+#pragma unroll 8
+            for (int y = 0; y < TY; y++) sum += part[y][c];
+            out.at<T>(row, hg, hi)[vb * COLS + c] = from_float<T>(sum * scale);
+        }
+        if (!again) break;
+        do row++;
+        while (row < rows && slot_of(row) != slot);
+        if (row >= rows) break;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int r = ty + i * TY;
+        if (mine && r < dk) {
+            if constexpr (VEC == 4)
+                __stcs(reinterpret_cast<float4 *>(state + r * states.row), make_float4(s[i][0], s[i][1], s[i][2], s[i][3]));
+            else
+                state[r * states.row] = s[i][0];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+static int sm_count() {
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+struct DecayPlan {
+    bool tc, split;
+    int64_t segment, slots;
+};
+
+static DecayPlan plan_of(const km_decay_problem &p) {
+    DecayPlan r;
+    r.tc = p.path == 2;
+    const int64_t chunk = r.tc ? 128 : FC, sms = 148, heads = p.groups * p.group;
+    const int64_t chunks = ceil_div(std::max<int64_t>(p.tokens, 1), chunk);
+    // Chunks of a segment.  A cut costs the segments' own states (k and v once more) and the scan, about half of the
+    // time again and some chunks' worth of launches.
+    int64_t per = chunks;
+    if (p.packed) {
+        // lengths are known on the device only: segments of which all sequences together give two per SM
+        per = std::min(chunks, std::max<int64_t>(4, ceil_div(chunks * heads, 2 * sms)));
+    } else {
+        double best = (double)ceil_div(p.sequences * heads, sms) * (double)chunks;
+        for (int64_t n = 2; n <= 64 && n <= chunks; n++) {
+            const int64_t len = ceil_div(chunks, n), pieces = ceil_div(chunks, len);
+            const double cost = (double)ceil_div(p.sequences * heads * pieces, sms) * (double)len * 1.5 + 8.0;
+            if (cost < best) best = cost, per = len;
+        }
+    }
+    r.segment = per * chunk;
+    r.split = per < chunks;
+    r.slots = p.packed ? p.tokens / r.segment + p.sequences : p.sequences * ceil_div(std::max<int64_t>(p.tokens, 1), r.segment);
+    return r;
+}
+
+static int check_problem(const char *name, const km_decay_problem *p) {
+    KM_REQUIRE(p != nullptr, KM_ERR_INVALID_ARGUMENT, "%s: null problem", name);
+    KM_REQUIRE(p->dtype >= KM_TYPE_F32 && p->dtype <= KM_TYPE_F16 && (p->out_dtype == p->dtype || p->out_dtype == KM_TYPE_F32),
+               KM_ERR_INVALID_ARGUMENT, "%s: bad element type", name);
+    KM_REQUIRE(p->path == 1 || (p->path == 2 && p->dtype != KM_TYPE_F32), KM_ERR_UNSUPPORTED,
+               "%s: path must be 1 (FMA pipe) or, for 16-bit types, 2 (tensor cores)", name);
+    KM_REQUIRE(p->sequences >= 0 && p->tokens >= 0 && p->groups >= 0 && p->group >= 1, KM_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
+    KM_REQUIRE(p->dk >= 1 && p->dk <= KM_DECAY_MAX_DIM && p->dv >= 1 && p->dv <= KM_DECAY_MAX_DIM, KM_ERR_UNSUPPORTED,
+               "%s: head sizes must be 1 to %d", name, KM_DECAY_MAX_DIM);
+    const int64_t limit = 1LL << 31;
+    KM_REQUIRE(p->tokens < limit && p->sequences < limit && p->groups < limit && p->group < limit &&
+                   p->groups * p->group < limit && p->sequences * (p->groups * p->group) < limit,
+               KM_ERR_UNSUPPORTED, "%s: more than 2^31 tokens or (sequence, head) pairs", name);
+    return KM_OK;
+}
+
+// What path 0 takes.
+static km_decay_problem resolved(const km_decay_problem &p) {
+    km_decay_problem r = p;
+    if (r.path == 0) r.path = 1;
+    return r;
+}
+
+template <typename T, typename O>
+static int launch_fma(const DecayArgs &a, bool state_only, cudaStream_t s) {
+    auto kernel = state_only ? decay_fma_kernel<T, O, true> : decay_fma_kernel<T, O, false>;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FMA_SMEM);
+    if (err != cudaSuccess) return cuda_fail(err, "decay_fma_kernel");
+    kernel<<<(unsigned)(a.slots * a.heads), 256, FMA_SMEM, s>>>(a);
+    KM_CHECK_LAUNCH("decay_fma_kernel launch");
+    return KM_OK;
+}
+
+static int launch_main(const km_decay_problem &p, const DecayArgs &a, bool tc, bool state_only, cudaStream_t s) {
+    if (tc) return launch_decay_tc(p, a, state_only, s);
+    const bool wide = p.out_dtype == KM_TYPE_F32;
+    if (p.dtype == KM_TYPE_F32) return launch_fma<float, float>(a, state_only, s);
+    if (p.dtype == KM_TYPE_BF16)
+        return wide ? launch_fma<__nv_bfloat16, float>(a, state_only, s) : launch_fma<__nv_bfloat16, __nv_bfloat16>(a, state_only, s);
+    return wide ? launch_fma<__half, float>(a, state_only, s) : launch_fma<__half, __half>(a, state_only, s);
+}
+
+static DecayArgs make_args(const km_decay_problem &p, const km_view *q, const km_view *k, const km_view *v, const float *log_decay,
+                           const int32_t *starts, const km_view *state_in) {
+    DecayArgs a = {};
+    a.q = make_operand(q), a.k = make_operand(k), a.v = make_operand(v);
+    a.state_in = make_operand(state_in);
+    a.log_decay = log_decay;
+    a.starts = p.packed ? starts : nullptr;
+    a.sequences = p.sequences, a.tokens = p.tokens, a.group = p.group, a.heads = p.groups * p.group;
+    a.dk = (int)p.dk, a.dv = (int)p.dv;
+    return a;
+}
+
+}  // namespace km
+
+extern "C" size_t km_decay_attention_workspace_bytes(const km_decay_problem *problem) {
+    using namespace km;
+    if (problem == nullptr) return 0;
+    const km_decay_problem p = resolved(*problem);
+    if (check_problem("km_decay_attention_workspace_bytes", &p) != KM_OK) return 0;
+    const DecayPlan plan = plan_of(p);
+    return plan.split ? (size_t)plan.slots * (size_t)(p.groups * p.group * p.dk * p.dv) * 4 : 0;
+}
+
+extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view *q, const km_view *k, const km_view *v, const km_view *out,
+                                  const float *log_decay, const int32_t *starts, const km_view *state_in, const km_view *state_out,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace km;
+    KM_REQUIRE(problem != nullptr, KM_ERR_INVALID_ARGUMENT, "km_decay_attention: null problem");
+    const km_decay_problem p = resolved(*problem);
+    int rc = check_problem("km_decay_attention", &p);
+    if (rc != KM_OK) return rc;
+    if (p.sequences == 0 || p.groups == 0) return KM_OK;
+    KM_REQUIRE(q && k && v && out && log_decay && (!p.packed || starts), KM_ERR_INVALID_ARGUMENT, "km_decay_attention: null argument");
+    KM_REQUIRE(p.tokens == 0 || (q->data && k->data && v->data && out->data), KM_ERR_INVALID_ARGUMENT, "km_decay_attention: null pointer");
+    const DecayPlan plan = plan_of(p);
+    const size_t need = km_decay_attention_workspace_bytes(problem);
+    KM_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KM_ERR_WORKSPACE,
+               "km_decay_attention: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
+    a.out = make_operand(out);
+    a.state_out = make_operand(state_out);
+    a.segment = plan.segment;
+    a.slots = plan.slots;
+    a.states = static_cast<float *>(workspace);
+    a.scale_in = p.reverse ? p.scale : 1.0f;
+    a.scale_out = p.reverse ? 1.0f : p.scale;
+    a.reverse = p.reverse != 0;
+    a.wait_polls = current_wait_polls();
+    a.gave_up = plan.tc ? gave_up_word() : nullptr;
+    KM_REQUIRE(a.slots * a.heads < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_attention: more than 2^31 work items");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (plan.split) {
+        rc = launch_main(p, a, plan.tc, true, s);
+        if (rc != KM_OK) return rc;
+        decay_scan_kernel<<<dim3((unsigned)(p.sequences * a.heads), 8), 256, 0, s>>>(a);
+        KM_CHECK_LAUNCH("decay_scan_kernel launch");
+    }
+    return launch_main(p, a, plan.tc, false, s);
+}
+
+extern "C" size_t km_decay_gradient_workspace_bytes(const km_decay_problem *problem) {
+    using namespace km;
+    if (problem == nullptr) return 0;
+    const km_decay_problem p = resolved(*problem);
+    if (check_problem("km_decay_gradient_workspace_bytes", &p) != KM_OK) return 0;
+    return (size_t)(p.sequences * p.groups * p.group) * (size_t)ceil_div(p.dv, GV) * sizeof(double);
+}
+
+extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view *q, const km_view *k, const km_view *v, const km_view *dout,
+                                 const float *log_decay, const int32_t *starts, const km_view *state_in, const km_view *dstate, float *grad,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace km;
+    KM_REQUIRE(problem != nullptr, KM_ERR_INVALID_ARGUMENT, "km_decay_gradient: null problem");
+    const km_decay_problem p = resolved(*problem);
+    int rc = check_problem("km_decay_gradient", &p);
+    if (rc != KM_OK) return rc;
+    if (p.groups == 0) return KM_OK;
+    KM_REQUIRE(q && k && v && dout && log_decay && grad && (!p.packed || starts), KM_ERR_INVALID_ARGUMENT, "km_decay_gradient: null argument");
+    const size_t need = km_decay_gradient_workspace_bytes(problem);
+    KM_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KM_ERR_WORKSPACE,
+               "km_decay_gradient: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
+    a.scale_in = 1.0f, a.scale_out = p.scale;
+    const Operand d = make_operand(dout), ds = make_operand(dstate);
+    const int vblocks = (int)ceil_div(p.dv, GV);
+    const int64_t ctas = p.sequences * a.heads * vblocks;
+    KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_gradient: more than 2^31 work items");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    double *partials = static_cast<double *>(workspace);
+    if (ctas > 0) {
+        auto kernel = p.dtype == KM_TYPE_F32    ? decay_gradient_kernel<float>
+                      : p.dtype == KM_TYPE_BF16 ? decay_gradient_kernel<__nv_bfloat16>
+                                                : decay_gradient_kernel<__half>;
+        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM);
+        if (err != cudaSuccess) return cuda_fail(err, "decay_gradient_kernel");
+        kernel<<<(unsigned)ctas, 256, GRAD_SMEM, s>>>(a, d, ds, vblocks, partials);
+        KM_CHECK_LAUNCH("decay_gradient_kernel launch");
+    }
+    decay_gradient_finish_kernel<<<(unsigned)a.heads, 256, 0, s>>>(p.sequences * vblocks, partials, grad);
+    KM_CHECK_LAUNCH("decay_gradient_finish_kernel launch");
+    return KM_OK;
+}
+
+extern "C" int km_group_sums(int32_t dtype, int64_t rows, int64_t groups, int64_t group, int64_t dim, const float *in, void *out, void *stream) {
+    using namespace km;
+    KM_REQUIRE(dtype >= KM_TYPE_F32 && dtype <= KM_TYPE_F16 && rows >= 0 && groups >= 0 && group >= 1 && dim >= 0, KM_ERR_INVALID_ARGUMENT,
+               "km_group_sums: bad arguments");
+    const int64_t count = rows * groups * dim;
+    if (count == 0) return KM_OK;
+    KM_REQUIRE(in && out, KM_ERR_INVALID_ARGUMENT, "km_group_sums: null pointer");
+    const unsigned ctas = (unsigned)std::min<int64_t>(ceil_div(count, 256), 8LL * sm_count());
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == KM_TYPE_F32)
+        group_sums_kernel<float><<<ctas, 256, 0, s>>>(count, group, dim, in, static_cast<float *>(out));
+    else if (dtype == KM_TYPE_BF16)
+        group_sums_kernel<__nv_bfloat16><<<ctas, 256, 0, s>>>(count, group, dim, in, static_cast<__nv_bfloat16 *>(out));
+    else
+        group_sums_kernel<__half><<<ctas, 256, 0, s>>>(count, group, dim, in, static_cast<__half *>(out));
+    KM_CHECK_LAUNCH("km_group_sums launch");
+    return KM_OK;
+}
+
+namespace km {
+
+template <typename T>
+static int launch_step(int64_t rows, int64_t pool, int64_t heads, int64_t group, int dk, int dv, const Operand &q, const Operand &k,
+                       const Operand &v, const Operand &out, const float *log_decay, const Operand &states, int slot_type,
+                       const void *slots, float scale, cudaStream_t s) {
+    // columns of 16 bytes where every row of every state starts on a boundary of 16 bytes
+    const bool wide = dv % 4 == 0 && reinterpret_cast<uintptr_t>(states.data) % 16 == 0 && states.seq % 4 == 0 && states.group % 4 == 0 &&
+                      states.head % 4 == 0 && states.row % 4 == 0;
+    // few rows: 32 columns to a CTA, so that more SMs share a state
+    const bool narrow = !wide || dv <= 32 || rows * heads < 4 * 148;
+    const int64_t ctas = rows * heads * ceil_div(dv, narrow ? 32 : 128);
+    KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_step: more than 2^31 work items");
+    auto kernel = !wide ? decay_step_kernel<T, 1, 32> : narrow ? decay_step_kernel<T, 4, 32> : decay_step_kernel<T, 4, 128>;
+    kernel<<<(unsigned)ctas, 256, 0, s>>>(rows, pool, heads, group, dk, dv, q, k, v, out, log_decay, states, slot_type, slots, scale);
+    KM_CHECK_LAUNCH("km_decay_step launch");
+    return KM_OK;
+}
+
+}  // namespace km
+
+extern "C" int km_decay_step(int32_t dtype, int64_t rows, int64_t pool, int64_t groups, int64_t group, int64_t dk, int64_t dv,
+                             const km_view *q, const km_view *k, const km_view *v, const km_view *out, const float *log_decay,
+                             const km_view *states, int32_t slot_type, const void *slots, float scale, void *stream) {
+    using namespace km;
+    KM_REQUIRE(dtype >= KM_TYPE_F32 && dtype <= KM_TYPE_F16 && rows >= 0 && pool >= 0 && groups >= 0 && group >= 1, KM_ERR_INVALID_ARGUMENT,
+               "km_decay_step: bad arguments");
+    KM_REQUIRE(dk >= 1 && dk <= KM_DECAY_MAX_DIM && dv >= 1 && dv <= KM_DECAY_MAX_DIM, KM_ERR_UNSUPPORTED,
+               "km_decay_step: head sizes must be 1 to %d", KM_DECAY_MAX_DIM);
+    KM_REQUIRE(slots == nullptr ? rows <= pool : (slot_type == KM_TYPE_I32 || slot_type == KM_TYPE_I64), KM_ERR_INVALID_ARGUMENT,
+               "km_decay_step: bad slots");
+    KM_REQUIRE(rows < (1LL << 31) && groups < (1LL << 31) && group < (1LL << 31) && groups * group < (1LL << 31), KM_ERR_UNSUPPORTED,
+               "km_decay_step: more than 2^31 rows or heads");
+    if (rows == 0 || groups == 0) return KM_OK;
+    KM_REQUIRE(q && k && v && out && log_decay && states && q->data && k->data && v->data && out->data, KM_ERR_INVALID_ARGUMENT,
+               "km_decay_step: null argument");
+    KM_REQUIRE(q->stride[1] == 1 && k->stride[1] == 1 && v->stride[1] == 1 && out->stride[1] == 1 && states->stride[1] == 1,
+               KM_ERR_INVALID_ARGUMENT, "km_decay_step: values of a head must be contiguous");
+    const Operand oq = make_operand(q), ok = make_operand(k), ov = make_operand(v), oo = make_operand(out), os = make_operand(states);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t heads = groups * group;
+    if (dtype == KM_TYPE_F32)
+        return launch_step<float>(rows, pool, heads, group, (int)dk, (int)dv, oq, ok, ov, oo, log_decay, os, slot_type, slots, scale, s);
+    if (dtype == KM_TYPE_BF16)
+        return launch_step<__nv_bfloat16>(rows, pool, heads, group, (int)dk, (int)dv, oq, ok, ov, oo, log_decay, os, slot_type, slots, scale, s);
+    return launch_step<__half>(rows, pool, heads, group, (int)dk, (int)dv, oq, ok, ov, oo, log_decay, os, slot_type, slots, scale, s);
+}

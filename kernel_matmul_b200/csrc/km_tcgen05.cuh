@@ -44,7 +44,7 @@ unsigned current_wait_polls();
 // (km_workspace_status) and one word per device in mapped host memory, which the host reads without
 // a copy or an event per launch (km_take_gave_up).  gave_up_word(): that word for the current
 // device, null if the mapping could not be made.  `what` is one of the codes below.
-enum GaveUp : int { GAVE_UP_MATMUL = 1, GAVE_UP_GRADIENT = 2 };
+enum GaveUp : int { GAVE_UP_MATMUL = 1, GAVE_UP_GRADIENT = 2, GAVE_UP_DECAY = 3 };
 int *gave_up_word();
 __device__ __forceinline__ void report_gave_up(int *status, int *word, int what) {
     atomicExch(status, 1);

@@ -28,7 +28,7 @@ void poll_gave_up(int device) {
     int32_t what = 0;
     raise_on(km_take_gave_up(device, &what));
     if (what != 0)
-        throw GaveUpError(std::string(what == 1 ? "matmul" : "gradient") +
+        throw GaveUpError(std::string(what == 1 ? "matmul" : what == 2 ? "gradient" : "decay_attention") +
                           ": a bounded wait inside the tensor-core kernel gave up (status word != 0); "
                           "the results of that call are invalid");
 }

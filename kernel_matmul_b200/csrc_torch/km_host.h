@@ -164,4 +164,18 @@ Tensor index_ad(int64_t kernel_type, const Tensor &x1, const Tensor &x2, const T
 std::pair<Tensor, Tensor> positive_params(const std::vector<Tensor> &raw, double lower_bound, int64_t lengthscales,
                                           std::optional<double> cutoff_factor);
 
+
+// The sequence operators, km_sequence.cpp.
+// q and k (k may be absent) turned by positions * frequencies; differentiable in q and k
+std::vector<Tensor> rotary(const Tensor &q, const std::optional<Tensor> &k, const Tensor &positions, const Tensor &frequencies,
+                           bool interleaved, double scale);
+// the result and, with return_state, the state after the last token; differentiable in q, k, v, log_decay and initial_state
+std::vector<Tensor> decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, std::optional<double> scale,
+                                    const std::optional<Tensor> &initial_state, const std::optional<Tensor> &starts, bool return_state,
+                                    int64_t path);
+Tensor decay_attention_step(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, const Tensor &states,
+                            std::optional<double> scale, const std::optional<Tensor> &slots);
+// 2-norm of the elements of all tensors; with max_norm they are scaled in place
+Tensor global_norm(const std::vector<Tensor> &tensors, std::optional<double> max_norm, double eps);
+
 }  // namespace kmh

@@ -161,6 +161,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             set("kernel_matmul_b200._lib", "KmError", e);
         } catch (const kmh::GaveUpError &e) {
             set("kernel_matmul_b200.ops", "KernelGaveUpError", e);
+        } catch (const kmh::ArgumentError &e) {
+            PyErr_SetString(PyExc_ValueError, e.what());
         }
     });
 
@@ -247,6 +249,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("dense_ad", &kmh::dense_ad, nogil());
     m.def("index_ad", &kmh::index_ad, nogil());
     m.def("positive_params", &kmh::positive_params, nogil());
+    m.def("rotary", &kmh::rotary, nogil());
+    m.def("decay_attention", &kmh::decay_attention, nogil());
+    m.def("decay_attention_step", &kmh::decay_attention_step, nogil());
+    m.def("global_norm", &kmh::global_norm, nogil());
     m.def("poll_gave_up", &kmh::poll_gave_up);
     m.def("band", &band, nogil());
     m.def("band_cutoffs", &band_cutoffs, nogil());

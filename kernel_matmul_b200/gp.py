@@ -86,12 +86,14 @@ class MllGradient:
 
 def mll_gradient(kernel_type: str, x: Tensor, params: Tensor, sigma2: float, y: Tensor, *, cutoff: float | None,
                  probes: Tensor | None = None, num_probes: int = 15, cg_iterations: int = 100, group=None,
-                 path: str = "auto") -> MllGradient:
+                 path: str = "auto", max_grad_norm: float | None = None) -> MllGradient:
     """Gradient of the negative log marginal likelihood wrt ``params`` (``(P,)``) and ``sigma2``.
 
     ``x (n,)`` sorted inputs and ``y (n,)`` targets on a CUDA device; ``probes (n, t)`` fixes the
     trace probes (default: ``num_probes`` Rademacher vectors from torch's current generator).
     With an initialised process group the CG products are sharded by rows over its ranks.
+    ``max_grad_norm``: bound on the norm of both gradients together (``ops.clip_global_norm_``): the trace part is a
+    stochastic estimate, of which a single step may be far off.
     """
     n = x.shape[-1]
     start, end = ranges.make_ranges(cutoff, x)
@@ -108,6 +110,8 @@ def mll_gradient(kernel_type: str, x: Tensor, params: Tensor, sigma2: float, y: 
     right = torch.cat([u.reshape(n, 1), probes], dim=-1).contiguous()
     grad_params = ops.bilinear_derivative(kernel_type, x, x, left, right, params, start, end, path=path)
     grad_sigma2 = -0.5 * (u * u).sum() + (0.5 / t) * (w * probes).sum()
+    if max_grad_norm is not None:
+        ops.clip_global_norm_([grad_params, grad_sigma2], max_grad_norm)
     inv_quad = (y * u).sum()
     # log det Khat from the Lanczos coefficients of the probe columns (columns 1 .. t of the solve)
     quad = _C.log_forms(res.alphas[:, 1:], res.betas[:, 1:], res.residual_norms[:, 1:], (probes * probes).sum(dim=0), 1e-7)

@@ -12,6 +12,7 @@ never materialised); gradients are produced for ``params`` only.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Sequence
 
 import torch
@@ -347,7 +348,114 @@ def count_entries(m: int, n: int, start: Tensor, end: Tensor) -> Tensor:
     return out
 
 
+# --------------------------------------------------------------------------- sequence operators
+
+
+def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                       original_tokens: int | None = None, fast_turns: float = 32.0, slow_turns: float = 1.0,
+                       device: torch.device | str | int | None = None) -> tuple[Tensor, float]:
+    """Angular frequencies ``base^(-2 i / dim)`` of the ``dim / 2`` pairs of a rotary embedding (float64, on ``device``, default:
+    the current CUDA device) and the factor for ``rotary(..., scale=)``.  Computed once, not per call.
+
+    ``scaling`` for contexts ``factor`` times as long as the ``original_tokens`` a model was trained on: ``"linear"`` divides all
+    frequencies by ``factor``; ``"base"`` raises the base so that the slowest pair is slowed by ``factor`` and the fastest not at
+    all; ``"parts"`` keeps pairs that turn ``fast_turns`` times or more over ``original_tokens``, slows those that turn
+    ``slow_turns`` times or less by ``factor`` and blends in between, with a factor of ``0.1 ln(factor) + 1`` on the values
+    (Peng et al. 2023, arXiv:2309.00071)."""
+    if dim < 0 or dim % 2:
+        raise ValueError(f"dim must be even and not negative, got {dim}")
+    if not base > 0.0 or not factor > 0.0:
+        raise ValueError("base and factor must be positive")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if scaling == "base" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    exponents = -torch.arange(0, dim, 2, dtype=torch.float64) / max(dim, 1)
+    frequencies, scale = torch.as_tensor(base, dtype=torch.float64) ** exponents, 1.0
+    if scaling == "linear":
+        frequencies = frequencies / factor
+    elif scaling == "parts":
+        if original_tokens is None or original_tokens <= 0 or not fast_turns > slow_turns:
+            raise ValueError("scaling 'parts' needs original_tokens > 0 and fast_turns > slow_turns")
+        turns = original_tokens * frequencies / (2.0 * math.pi)
+        keep = ((turns - slow_turns) / (fast_turns - slow_turns)).clamp(0.0, 1.0)
+        frequencies = frequencies * keep + frequencies / factor * (1.0 - keep)
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return frequencies.to("cuda" if device is None else device), scale
+
+
+def rotary(q: Tensor, k: Tensor | None, positions: Tensor, frequencies: Tensor, *, interleaved: bool = False,
+           scale: float = 1.0) -> tuple[Tensor, Tensor | None]:
+    """Rotary positions: ``q`` and ``k`` (``(*batch, tokens, heads, dim)``, their own numbers of heads; fp32, bf16 or fp16; any
+    strides) with every pair of a head's first ``2 len(frequencies)`` values turned by ``position * frequency`` and multiplied by
+    ``scale``; the values behind them are copied.  Pairs are ``(i, i + len(frequencies))`` or, ``interleaved``,
+    ``(2 i, 2 i + 1)``.  One launch for both.
+
+    ``positions``: ``(tokens,)`` or broadcastable to ``(*batch, tokens)``, int32, int64 or fp32 (times need not be whole).
+    ``frequencies``: fp32 or fp64, e.g. from ``rotary_frequencies``.  Angles are evaluated in 64 bits, values in 32, rounded once.
+    Differentiable in ``q`` and ``k`` (any number of times)."""
+    _is_cuda(q, positions, frequencies, *(() if k is None else (k,)))
+    out = _C.rotary(q, k, positions, frequencies, interleaved, scale)
+    return out[0], (out[1] if k is not None else None)
+
+
+_DECAY_PATHS = {"auto": 0, "fma": 1, "tc": 2}
+
+
+def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scale: float | None = None,
+                    initial_state: Tensor | None = None, sequence_starts: Tensor | None = None, return_state: bool = False,
+                    path: str = "auto") -> Tensor | tuple[Tensor, Tensor]:
+    """Linear attention with a decay for each head: the product of the causal matrix ``scale e^(g (t - s)) <q_t, k_s>``, ``s <= t``,
+    which is generated on the fly, with ``v``; ``g = log_decay[head]``.  As a recurrence over a state ``S`` ``(dk, dv)``:
+    ``S_t = e^g S_(t-1) + k_t v_t^T``, ``out_t = scale S_t^T q_t``.
+
+    ``q (*batch, tokens, heads, dk)``, ``k (*batch, tokens, groups, dk)``, ``v (*batch, tokens, groups, dv)`` with ``heads`` a
+    multiple of ``groups`` (head ``h`` reads group ``h // (heads // groups)``); fp32, bf16 or fp16, any strides, ``dk`` and ``dv``
+    up to 128; ``log_decay (heads,)`` fp32, ``-inf`` to 0 (0: no decay; growing states are not refused).  ``scale``: default
+    ``dk ** -0.5``.  Returns ``(*batch, tokens, heads, dv)`` and, with ``return_state``, the states after the last token
+    ``(*batch, heads, dk, dv)`` in fp32, which ``initial_state`` of a later call, or ``decay_attention_step``, goes on from.
+
+    ``sequence_starts``: int32 ``(sequences + 1,)`` on the device, not decreasing: sequence ``i`` is the rows
+    ``[starts[i], starts[i + 1])`` of ``q (tokens, heads, dk)`` etc., empty ones included; rows of no sequence get zeros (and
+    have no gradient).  States then are ``(sequences, heads, dk, dv)``.  The values are read on the device and clamped to the rows there are.
+
+    Differentiable once in ``q``, ``k``, ``v``, ``log_decay`` and ``initial_state``.  ``path``: ``"fma"``, ``"tc"`` (tensor
+    cores, 16-bit operands) or ``"auto"``.  A value that is not finite spoils its sequence's results from up to 127 tokens before
+    it on (the block in which it is multiplied), and no other sequence's or head's."""
+    _is_cuda(q, k, v, log_decay)
+    if path not in _DECAY_PATHS:
+        raise ValueError(f"unknown path {path!r}")
+    out = _C.decay_attention(q, k, v, log_decay, scale, initial_state, sequence_starts, return_state, _DECAY_PATHS[path])
+    return (out[0], out[1]) if return_state else out[0]
+
+
+def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, states: Tensor, *, scale: float | None = None,
+                         slots: Tensor | None = None) -> Tensor:
+    """One more token for each of many sequences: ``decay_attention``'s recurrence once, ``states`` updated in place.
+
+    ``q (rows, heads, dk)``, ``k (rows, groups, dk)``, ``v (rows, groups, dv)``; ``states (slots, heads, dk, dv)`` fp32 with a
+    contiguous last dim.  ``slots`` (int32 or int64 ``(rows,)`` on the device): the state of each row; default: row ``i`` has
+    state ``i``.  A row whose slot is not in ``[0, len(states))`` (padding of a batch) gets zeros and touches no state; rows
+    with the same slot are tokens of one sequence, in their order.  Returns ``(rows, heads, dv)``.  No gradient."""
+    _is_cuda(q, k, v, log_decay, states)
+    return _C.decay_attention_step(q, k, v, log_decay, states, scale, slots)
+
+
+def global_norm(tensors: Sequence[Tensor]) -> Tensor:
+    """2-norm of the elements of all ``tensors`` (fp32, bf16, fp16, on one CUDA device) as a 0-dim fp32 tensor; one pass, no
+    synchronisation, the same bits for the same tensors.  A tensor that is listed twice counts once."""
+    return _C.global_norm(list(tensors), None, 0.0)
+
+
+def clip_global_norm_(tensors: Sequence[Tensor], max_norm: float, *, eps: float = 1e-6) -> Tensor:
+    """``global_norm`` of the gradients ``tensors``, which are multiplied in place by ``min(1, max_norm / (norm + eps))``.  Returns
+    the norm before.  Where that factor is one the tensors are not written; a norm that is not finite gives what the formula
+    gives.  Tensors that overlap in part are refused."""
+    return _C.global_norm(list(tensors), float(max_norm), float(eps))
+
+
 __all__ = [
+    "rotary", "rotary_frequencies", "decay_attention", "decay_attention_step", "global_norm", "clip_global_norm_",
     "matmul", "matmul_rows", "prepare_matmul_rows", "PreparedRowsProduct", "tc_status", "check", "used_tensor_cores", "KernelGaveUpError", "matmul_bwd", "bilinear_derivative", "dense", "dense_bwd", "index", "index_bwd",
     "count_entries", "BLOCK_SIZE", "NUM_PARAMS",
 ]
