@@ -554,7 +554,7 @@ static int check_problem(const char *name, const km_decay_problem *p) {
 // What path 0 takes.
 static km_decay_problem resolved(const km_decay_problem &p) {
     km_decay_problem r = p;
-    if (r.path == 0) r.path = 1;
+    if (r.path == 0) r.path = r.dtype == KM_TYPE_F32 ? 1 : 2;
     return r;
 }
 

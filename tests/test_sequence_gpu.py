@@ -35,7 +35,7 @@ def starts_of(lengths, first=0):
 
 
 def paths(dtype):
-    return ["fma"]
+    return ["fma"] if dtype == torch.float32 else ["fma", "tc"]
 
 
 CASES = [
