@@ -16,7 +16,7 @@ constexpr int FMA_SMEM = (3 * FC * FLD + FC * 36 + KM_DECAY_MAX_DIM * KM_DECAY_M
 
 template <typename T>
 __device__ __forceinline__ void load_chunk(float *dst, const DecayArgs &a, const Segment &s, const Operand &o, int64_t hg, int64_t hi,
-                                           int64_t first, int tokens, int dim, int ld, int width) {
+                                           int first, int tokens, int dim, int ld, int width) {
     const T *src = o.at<T>(a.starts == nullptr ? s.seq : 0, hg, hi);
     for (int i = threadIdx.x; i < FC * width; i += blockDim.x) {
         const int t = i / width, c = i - t * width;
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
             for (int j = 0; j < 8; j++) z[i][j] *= w;
     }
 
-    for (int64_t first = s.first; first < s.first + s.count; first += FC) {
-        const int tokens = (int)min((int64_t)FC, s.first + s.count - first);
+    for (int first = s.first; first < s.first + s.count; first += FC) {
+        const int tokens = min(FC, s.first + s.count - first);
         const bool final = first + tokens == s.length;
         const int e = final && !a.reverse ? tokens - 1 : tokens;
         __syncthreads();
@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// States at the start of each segment, in place: states[slot] held the segment's own contribution.  The segments of a
-// sequence one after the other, its values spread over 8 x 256 threads: each value is read and written once.
+// States at the start of each segment, in place: states[slot] held the segment's own contribution.  A thread takes one
+// value of the state through the segments of a sequence, eight of them loaded ahead: read and written once.
 __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
     const int64_t h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
@@ -209,21 +209,26 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
     if (n <= 1) return;
     const float g2 = log2_decay(a.log_decay[h]);
     const float carry = exp2f(g2 * (float)a.segment), enter = a.reverse ? 1.0f : exp2f(g2);
-    const int values = a.dk * a.dv;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < values; i += 256 * gridDim.y) {
-        float zv = 0.0f;
-        if (a.state_in.data != nullptr)
-            zv = enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col];
-        float *p = a.states + (slot0 * a.heads + h) * (int64_t)values + i;
-        const int64_t step = a.heads * (int64_t)values;
-        float own = *p;
-        for (int64_t j = 1; j < n; j++) {
-            p += step;
-            zv = fmaf(carry, zv, own);
-            own = j + 1 < n ? *p : 0.0f;
-            *p = zv;
+    const int values = a.dk * a.dv, i = blockIdx.y * 256 + threadIdx.x;
+    if (i >= values) return;
+    float zv = 0.0f;
+    if (a.state_in.data != nullptr)
+        zv = enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col];
+    float *p = a.states + (slot0 * a.heads + h) * (int64_t)values + i;
+    const int64_t step = a.heads * (int64_t)values;
+    for (int64_t j = 0; j + 1 < n; j += 8) {
+        float own[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) own[u] = j + u + 1 < n ? p[(j + u) * step] : 0.0f;
+        // (states[j] itself is the state at its start; what is left in it by the group before has been read here)
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            if (j + u > 0 && j + u < n) p[(j + u) * step] = zv;
+            zv = fmaf(carry, zv, own[u]);
         }
     }
+    // (the last group may have ended right before the last segment)
+    if ((n - 1) % 8 == 0) p[(n - 1) * step] = zv;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -245,8 +250,9 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
     const int64_t rest = blockIdx.x / vblocks, h = rest % a.heads, seq = rest / a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
     Segment s = {};
-    s.seq = seq;
-    sequence_rows(a, seq, s.begin, s.length);
+    int64_t begin, length;
+    sequence_rows(a, seq, begin, length);
+    s.seq = (int)seq, s.begin = (int)begin, s.length = (int)length;
     const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;  // columns 4 tx .. + 3, rows ty + 32 i
     const int cols = min(GV, a.dv - vb * GV), dk4 = (a.dk + 3) & ~3;
     const float g2 = log2_decay(a.log_decay[h]);
@@ -265,8 +271,8 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
             z[i][j] = m[i][j] = x;
         }
     double total = 0.0;
-    for (int64_t first = 0; first < s.length; first += FC) {
-        const int tokens = (int)min((int64_t)FC, s.length - first);
+    for (int first = 0; first < s.length; first += FC) {
+        const int tokens = min(FC, s.length - first);
         const int e = first + tokens == s.length ? tokens - 1 : tokens;
         __syncthreads();
         load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
@@ -522,10 +528,10 @@ static DecayPlan plan_of(const km_decay_problem &p) {
         // lengths are known on the device only: segments of which all sequences together give two per SM
         per = std::min(chunks, std::max<int64_t>(4, ceil_div(chunks * heads, 2 * sms)));
     } else {
-        double best = (double)ceil_div(p.sequences * heads, sms) * (double)chunks;
+        double best = (double)ceil_div(p.sequences * heads, sms) * (double)(chunks + 2);
         for (int64_t n = 2; n <= 64 && n <= chunks; n++) {
             const int64_t len = ceil_div(chunks, n), pieces = ceil_div(chunks, len);
-            const double cost = (double)ceil_div(p.sequences * heads * pieces, sms) * (double)len * 1.5 + 8.0;
+            const double cost = (double)ceil_div(p.sequences * heads * pieces, sms) * (double)(len + 2) * 1.5 + 6.0;
             if (cost < best) best = cost, per = len;
         }
     }
@@ -544,7 +550,7 @@ static int check_problem(const char *name, const km_decay_problem *p) {
     KM_REQUIRE(p->sequences >= 0 && p->tokens >= 0 && p->groups >= 0 && p->group >= 1, KM_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
     KM_REQUIRE(p->dk >= 1 && p->dk <= KM_DECAY_MAX_DIM && p->dv >= 1 && p->dv <= KM_DECAY_MAX_DIM, KM_ERR_UNSUPPORTED,
                "%s: head sizes must be 1 to %d", name, KM_DECAY_MAX_DIM);
-    const int64_t limit = 1LL << 31;
+    const int64_t limit = (1LL << 31) - 4096;
     KM_REQUIRE(p->tokens < limit && p->sequences < limit && p->groups < limit && p->group < limit &&
                    p->groups * p->group < limit && p->sequences * (p->groups * p->group) < limit,
                KM_ERR_UNSUPPORTED, "%s: more than 2^31 tokens or (sequence, head) pairs", name);
@@ -631,7 +637,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     if (plan.split) {
         rc = launch_main(p, a, plan.tc, true, s);
         if (rc != KM_OK) return rc;
-        decay_scan_kernel<<<dim3((unsigned)(p.sequences * a.heads), 8), 256, 0, s>>>(a);
+        decay_scan_kernel<<<dim3((unsigned)(p.sequences * a.heads), (unsigned)ceil_div(p.dk * p.dv, 256)), 256, 0, s>>>(a);
         KM_CHECK_LAUNCH("decay_scan_kernel launch");
     }
     return launch_main(p, a, plan.tc, false, s);

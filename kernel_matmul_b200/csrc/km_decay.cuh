@@ -70,10 +70,9 @@ __device__ __forceinline__ float log2_decay(float g) {
 }
 
 struct Segment {
-    int64_t seq, begin, length;  // its sequence: number, first row, rows
-    int64_t first, count;        // its tokens inside the sequence (in the order in which they are gone through)
-    int64_t slot;
-    int64_t spare, spares;       // rows of no sequence are shared by `spares` CTAs per head, of which this is number `spare`; -1: none
+    int seq, begin, length;  // its sequence: number, first row, rows (of all three there are less than 2^31)
+    int first, count;        // its tokens inside the sequence (in the order in which they are gone through)
+    int spare, spares;       // rows of no sequence are shared by `spares` CTAs per head, of which this is number `spare`; -1: none
     bool used, last;
 };
 
@@ -111,12 +110,11 @@ __device__ __forceinline__ int64_t segments_before(const DecayArgs &a, int64_t s
 // Segment number `slot` (one warp calls it, all lanes get the result).
 __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot) {
     Segment r = {};
-    r.slot = slot;
     r.spare = -1;
     int64_t index = 0;
     if (a.starts == nullptr) {
         const int64_t per = segments_of(a, a.tokens);
-        r.seq = slot / per;
+        r.seq = (int)(slot / per);
         index = slot - r.seq * per;
         r.used = true;
     } else {
@@ -139,30 +137,31 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot
             const unsigned hit = __ballot_sync(0xffffffffu, slot < upto);
             if (hit != 0) {
                 const int who = __ffs(hit) - 1;
-                r.seq = base + who;
+                r.seq = (int)base + who;
                 index = slot - __shfl_sync(0xffffffffu, upto - n, who);
                 r.used = true;
             }
             before = __shfl_sync(0xffffffffu, upto, 31);
         }
         if (!r.used) {
-            r.spare = slot - before;
-            r.spares = a.slots - before;
+            r.spare = (int)(slot - before);
+            r.spares = (int)(a.slots - before);
             return r;
         }
     }
-    sequence_rows(a, r.seq, r.begin, r.length);
-    const int64_t n = segments_of(a, r.length);
-    r.first = index * a.segment;
-    r.last = index == n - 1;
-    r.count = min(r.length - r.first, a.segment);
+    int64_t begin, length;
+    sequence_rows(a, r.seq, begin, length);
+    r.begin = (int)begin, r.length = (int)length;
+    r.first = (int)(index * a.segment);
+    r.last = index == segments_of(a, length) - 1;
+    r.count = (int)min(length - r.first, a.segment);
     // the very last slot is in use: its CTA sees to the rows of no sequence
     if (a.starts != nullptr && slot == a.slots - 1) r.spare = 0, r.spares = 1;
     return r;
 }
 
 // Row of the tensors that holds token i (in the order in which the sequence is gone through).
-__device__ __forceinline__ int64_t token_row(const DecayArgs &a, const Segment &s, int64_t i) {
+__device__ __forceinline__ int64_t token_row(const DecayArgs &a, const Segment &s, int i) {
     return s.begin + (a.reverse ? s.length - 1 - i : i);
 }
 

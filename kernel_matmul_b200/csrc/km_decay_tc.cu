@@ -15,8 +15,9 @@
 //
 // Bound by memory: a chunk of a head with dk = dv = 128 moves 128 KB and takes five products of 128^3 (1300 cycles of the tensor
 // pipe), while its share of HBM takes 5600 cycles.  So everything is about keeping loads in flight: two stages of Q, K, V (96 KB
-// each), each filled by a warp of its own through cp.async, which takes any row stride and zero-fills the rows behind
-// the last token; K~ goes over K and Q once S and QZ have read them, P over S.
+// each), filled through TMA; K~ goes over K and Q once S and QZ have read them, P over S.
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "km_decay.cuh"
@@ -25,26 +26,39 @@ namespace km {
 
 namespace {
 
-constexpr int TC = 128;            // tokens of a chunk
-constexpr int COMPUTE = 256;       // threads: two per lane of tensor memory
-constexpr int LOADERS = 32;        // threads per stage
-constexpr int THREADS = COMPUTE + 32 + 2 * LOADERS;
+constexpr int TC = 128;       // tokens of a chunk
+constexpr int GROUP = 256;    // threads of a group: two per lane of tensor memory
+// warps 0 - 7: results and state; 8 - 15: operands; 16: matrix products; 17, 18: loads; 19: none
+constexpr int MMA_WARP = 16, THREADS = 640;
+// Registers: 640 threads are launched with 96 each, 61 440 in all, which the groups divide: 256 x 128 + 256 x 72 + 128 x 80.
+constexpr int RESULT_REGS = 144, OPERAND_REGS = 64, OTHER_REGS = 64;
+static_assert(256 * RESULT_REGS + 256 * OPERAND_REGS + 128 * OTHER_REGS <= THREADS * 96, "registers at launch");
 constexpr int BLOCK_BYTES = TC * 128;  // 128 rows of 64 values
+
+// Tiles hold rows in the order of memory, in the reverse form too, which goes through the chunks from the last: row `m` of
+// a chunk of n tokens is token m, or token n - 1 - m in the order in which the sequence is gone through.
+__device__ __forceinline__ int chunk_row(const DecayArgs &a, const Segment &s, int chunk, int tokens) {
+    const int first = s.first + chunk * TC;
+    return s.begin + (a.reverse ? s.length - first - tokens : first);
+}
 
 template <int KB, int VB>
 struct Smem {
-    static constexpr int Q = 0, K = KB * BLOCK_BYTES, V = 2 * KB * BLOCK_BYTES, STAGE = (2 * KB + VB) * BLOCK_BYTES;
+    // (the Q tile is also where the results leave through: 8 warps' 4 KB)
+    static constexpr int Q = 0, K = 2 * BLOCK_BYTES, V = K + KB * BLOCK_BYTES, STAGE = V + VB * BLOCK_BYTES;
     static constexpr int Z = 2 * STAGE;                       // KB blocks of (64 VB rows of 64 values)
     static constexpr int REST = Z + KB * VB * 64 * 128;
     static constexpr int BYTES = 1024 + REST;
 };
 
 struct Control {
-    uint64_t full[2], empty[2], s_full, qz_full, p_ready, o_full, z_ready, drain, meet;
+    uint64_t full[2], empty[2], q_empty[2], s_full, qz_full, p_ready, o_full, z_ready, drain, meet[2];
     uint32_t tmem;
     int dead;
+    float inner[16];                // decays 2^(g2 (15 - j)), reverse 2^(g2 j)
+    __nv_bfloat16 p_scale[2][TC];   // fp16: power of two that takes the scaling of P's row back, by parity of the chunk
     __nv_bfloat16 z_scale[2][128];  // fp16: power of two that takes the scaling of Z's row back, by parity of the chunk
-    float row_max[2][TC];           // fp16: largest of a row in each half
+    uint8_t row_max[2][2][TC];      // fp16: exponent of a row's largest magnitude in each half, for either group
 };
 
 // tensor memory columns
@@ -92,6 +106,13 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
                  : "memory");
 }
 
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :
+                 : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 // two values as one word, the first in the low half, rounded to nearest
 template <typename T>
 __device__ __forceinline__ uint32_t pack(float a, float b);
@@ -116,42 +137,19 @@ __device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
     return __half22float2(reinterpret_cast<const __half2 &>(w));
 }
 
-// 2^n that brings a largest magnitude m to [2^13, 2^14) (fp16's range and as many of its small values as possible); 1 for 0 and
+// 2^n that brings a largest magnitude of (biased) exponent e to [2^13, 2^14) (fp16's range and as many of its small values as possible); 1 for 0 and
 // for what is not finite
-__device__ __forceinline__ float fp16_scale(float m) {
-    const int e = (int)((__float_as_uint(m) >> 23) & 0xffu);
+__device__ __forceinline__ int exponent_of(float m) { return (int)((__float_as_uint(m) >> 23) & 0xffu); }
+__device__ __forceinline__ float fp16_scale(int e) {
     if (e == 0 || e == 255) return 1.0f;
     return __uint_as_float((uint32_t)min(max(127 + 13 - (e - 127), 2), 252) << 23);  // (its inverse is a normal number too)
 }
 
-// One operand's rows into the stage, by the threads of the stage.
-template <typename T, int BLOCKS>
-__device__ __forceinline__ void load_tile(unsigned char *tile, const DecayArgs &a, const Segment &s, const Operand &o, int64_t hg,
-                                          int64_t hi, int64_t first, int tokens, int dim, bool aligned, int tid) {
-    constexpr int PIECES = BLOCKS * 8;  // of 16 bytes, in a row
-    const T *src = o.at<const T>(a.starts == nullptr ? s.seq : 0, hg, hi);
-    const int c = tid % PIECES, left = min(max(dim - c * 8, 0), 8);
-    unsigned char *to = tile + (c >> 3) * BLOCK_BYTES;
-    const int64_t step = (a.reverse ? -1 : 1) * o.row;
-    const T *p = src + token_row(a, s, first) * o.row + (int64_t)c * 8 * o.col;
-    for (int row = tid / PIECES; row < TC; row += LOADERS / PIECES) {
-        unsigned char *dst = to + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        const bool here = row < tokens && left > 0;
-        const T *from = here ? p + row * step : src;
-        if (aligned) {
-            const unsigned bytes = here ? left * 2u : 0u;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(from), "r"(bytes) : "memory");
-        } else {
-            union {
-                T v[8];
-                uint4 w;
-            } x;
-            x.w = make_uint4(0, 0, 0, 0);
-            if (here)
-                for (int j = 0; j < left; j++) x.v[j] = from[j * o.col];
-            *reinterpret_cast<uint4 *>(dst) = x.w;
-        }
-    }
+// The swizzle of rows of PITCH bytes, 128 or 64, on an offset from a boundary of 1024 bytes.
+template <int PITCH>
+__device__ __forceinline__ int swizzled(int offset) {
+    static_assert(PITCH == 128 || PITCH == 64, "a row is as wide as the swizzle");
+    return offset ^ (((offset >> 7) & (PITCH / 16 - 1)) << 4);
 }
 
 // Whether every row starts on a boundary of 16 bytes.
@@ -159,10 +157,59 @@ __device__ __forceinline__ bool rows_aligned(const Operand &o, int size) {
     return o.col == 1 && ((reinterpret_cast<uintptr_t>(o.data) | (uintptr_t)((o.seq | o.group | o.head | o.row) * size)) & 15) == 0;
 }
 
+// Tensor maps of q, k, v (boxes of 64 values x 128 tokens) and the result (up to 128 bytes x 32 tokens), and which operands have
+// one; the coordinates of a head and a sequence in them.
+struct Maps {
+    CUtensorMap q, k, v, out;
+    int use[4], by_group[4], by_head[4], by_seq[4];
+};
+
+__device__ __forceinline__ void tma_load(unsigned char *dst, const CUtensorMap &map, int x, int head, int row, int seq, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            smem_u32(dst)),
+        "l"(&map), "r"(x), "r"(head), "r"(row), "r"(seq), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_store(const CUtensorMap &map, int x, int head, int row, int seq, const unsigned char *src) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(&map), "r"(x), "r"(head), "r"(row),
+                 "r"(seq), "r"(smem_u32(src))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Shared memory that this thread's stores read may be written again.
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// Rows [0, tokens) of a tile without a tensor map (rows or values that do not lie on boundaries of 16 bytes), by a warp; zeros
+// behind them.  `src` is the head's value (row `first`, 0).
+template <typename T, int BLOCKS>
+__device__ __noinline__ void copy_tile(unsigned char *tile, const T *src, int64_t row, int64_t col, int tokens, int dim, int lane) {
+    constexpr int PIECES = BLOCKS * 8;
+    for (int i = lane; i < TC * PIECES; i += 32) {
+        const int r = i / PIECES, c = i % PIECES;
+        union {
+            T v[8];
+            uint4 w;
+        } x;
+        x.w = make_uint4(0, 0, 0, 0);
+        if (r < tokens)
+            for (int j = 0; j < min(dim - c * 8, 8); j++) x.v[j] = src[r * row + (c * 8 + j) * col];
+        *reinterpret_cast<uint4 *>(tile + (c >> 3) * BLOCK_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x.w;
+    }
+}
+
+// NaN into columns [c0, c1) of rows [first, end), by a warp.
+template <typename O>
+__device__ __noinline__ void poison_rows(O *out, int64_t row, int64_t col, int first, int end, int c0, int c1) {
+    for (int i = first + (threadIdx.x & 31); i < end; i += 32)
+        for (int c = c0; c < c1; c++) out[i * row + c * col] = from_float<O>(__int_as_float(0x7fc00000));
+}
+
 }  // namespace
 
 template <typename T, typename O, int KB, int VB, bool STATE_ONLY>
-__global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(DecayArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_constant__ DecayArgs a, const __grid_constant__ Maps maps) {
     using L = Smem<KB, VB>;
     constexpr bool HALF = std::is_same<T, __half>::value;
     constexpr int NZ = KB * 32;  // of the state's row: this thread's columns
@@ -177,42 +224,81 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(DecayArgs a) {
     if (!STATE_ONLY && s.spare >= 0) clear_spare_rows<O>(a, s, hg, hi);
     if (!s.used || (STATE_ONLY && s.last)) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int chunks = (int)((s.count + TC - 1) / TC);
+    const int chunks = (s.count + TC - 1) / TC;
 
     if (tid == 0) {
         for (int b = 0; b < 2; b++) {
-            mbar_init(&ctl.full[b], LOADERS);
+            mbar_init(&ctl.full[b], STATE_ONLY ? 33 : 34);  // the loading warp's lanes, and its byte counts
             mbar_init(&ctl.empty[b], 1);
+            mbar_init(&ctl.q_empty[b], GROUP);
+            mbar_init(&ctl.meet[b], GROUP);
         }
         mbar_init(&ctl.s_full, 1), mbar_init(&ctl.qz_full, 1), mbar_init(&ctl.o_full, 1), mbar_init(&ctl.drain, 1);
-        mbar_init(&ctl.p_ready, COMPUTE), mbar_init(&ctl.z_ready, COMPUTE), mbar_init(&ctl.meet, COMPUTE);
+        mbar_init(&ctl.p_ready, GROUP), mbar_init(&ctl.z_ready, GROUP);
         ctl.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == COMPUTE / 32) tmem_alloc(&ctl.tmem, 512);
+    const float g2 = log2_decay(a.log_decay[h]);
+    if (warp == MMA_WARP) tmem_alloc(&ctl.tmem, 512);
+    if (warp == MMA_WARP + 1 && lane < 16) ctl.inner[lane] = exp2f(g2 * (float)(a.reverse ? lane : 15 - lane));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
     const uint32_t base = smem_u32(smem);
-    const float g2 = log2_decay(a.log_decay[h]);
+    // this thread's lane of tensor memory and half of the columns (of the two groups of eight warps)
+    const int row = (warp & 3) * 32 + lane, half = (warp >> 2) & 1;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    const int group = warp >> 3;
+    // all threads of a group meet (false: gave up)
+    unsigned meetings = 0;
+    const auto meet = [&]() {
+        mbar_arrive(&ctl.meet[group]);
+        return mbar_wait_warp(&ctl.meet[group], meetings++ & 1, a.wait_polls);
+    };
 
-    if (warp > COMPUTE / 32) {  // ---------------------------------------------------------------- loads
-        const int ltid = tid - COMPUTE - 32, b = ltid / LOADERS, mine = ltid % LOADERS;
+    if (warp >= MMA_WARP) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    }
+    if (warp > MMA_WARP + 2) {
+    } else if (warp > MMA_WARP) {  // ---------------------------------------------------------------- loads
+        const int b = warp - MMA_WARP - 1;
         unsigned char *stage = smem + b * L::STAGE;
-        const bool aq = rows_aligned(a.q, 2), ak = rows_aligned(a.k, 2), av = rows_aligned(a.v, 2);
-        for (int it = b; it < chunks; it += 2) {
-            if (it >= 2 && !mbar_wait_warp(&ctl.empty[b], ((it >> 1) + 1) & 1, a.wait_polls)) break;
-            const int64_t first = s.first + (int64_t)it * TC;
-            const int tokens = (int)min((int64_t)TC, s.first + s.count - first);
-            load_tile<T, KB>(stage + L::K, a, s, a.k, hg, hi, first, tokens, a.dk, ak, mine);
-            if (!STATE_ONLY) load_tile<T, KB>(stage + L::Q, a, s, a.q, hg, hi, first, tokens, a.dk, aq, mine);
-            load_tile<T, VB>(stage + L::V, a, s, a.v, hg, hi, first, tokens, a.dv, av, mine);
-            asm volatile("cp.async.wait_all;" ::: "memory");
+        const int seq = a.starts == nullptr ? s.seq : 0;
+        const auto fetch = [&](auto blocks, int which, const CUtensorMap &map, const Operand &o, unsigned char *tile, int row0, int tokens, int dim) {
+            constexpr int BLOCKS = decltype(blocks)::value;
+            if (maps.use[which]) {
+                const int head = maps.by_group[which] * (int)hg + maps.by_head[which] * (int)hi;
+                if (lane == 0)
+                    for (int x = 0; x < BLOCKS; x++) tma_load(tile + x * BLOCK_BYTES, map, x * 64, head, row0, maps.by_seq[which] * seq, &ctl.full[b]);
+            } else {
+                copy_tile<T, BLOCKS>(tile, o.at<const T>(seq, hg, hi) + (int64_t)row0 * o.row, o.row, o.col, tokens, dim, lane);
+            }
+        };
+        using Keys = std::integral_constant<int, KB>;
+        using Values = std::integral_constant<int, VB>;
+        const unsigned kv_bytes = ((maps.use[1] ? KB : 0) + (maps.use[2] ? VB : 0)) * BLOCK_BYTES, q_bytes = (maps.use[0] ? KB : 0) * BLOCK_BYTES;
+        int filled = 0;
+        bool ok = true;
+        for (int it = b; it < chunks && ok; it += 2, filled++) {
+            ok = it < 2 || mbar_wait_warp(&ctl.empty[b], ((it >> 1) + 1) & 1, a.wait_polls);
+            if (!ok) break;
+            const int tokens = min(TC, s.count - it * TC), row0 = chunk_row(a, s, it, tokens);
+            if (lane == 0) mbar_expect_tx(&ctl.full[b], kv_bytes);
+            fetch(Keys(), 1, maps.k, a.k, stage + L::K, row0, tokens, a.dk);
+            fetch(Values(), 2, maps.v, a.v, stage + L::V, row0, tokens, a.dv);
+            if (!STATE_ONLY) {
+                ok = it < 2 || mbar_wait_warp(&ctl.q_empty[b], ((it >> 1) + 1) & 1, a.wait_polls);
+                if (!ok) *reinterpret_cast<volatile int *>(&ctl.dead) = 1;  // (before the others can see this stage as full)
+                if (lane == 0) mbar_expect_tx(&ctl.full[b], ok ? q_bytes : 0u);
+                if (ok) fetch(Keys(), 0, maps.q, a.q, stage + L::Q, row0, tokens, a.dk);
+            }
             fence_async_smem();
             mbar_arrive(&ctl.full[b]);
         }
-    } else if (warp == COMPUTE / 32) {  // ------------------------------------------------------------- matrix products
+        // no copy may be in flight when the CTA ends
+        if (filled > 0) mbar_wait_warp(&ctl.full[b], (filled - 1) & 1, TC_WAIT_POLLS);
+    } else if (warp == MMA_WARP) {  // ------------------------------------------------------------- matrix products
         constexpr uint32_t type = HALF ? 0u : 1u;
         constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);
         constexpr uint32_t idesc_s = idesc0 | ((128u >> 3) << 17);
@@ -222,15 +308,17 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(DecayArgs a) {
         bool ok = true;
         for (int it = 0; it < chunks && ok; it++) {
             const int b = it & 1;
-            const uint32_t q = base + b * L::STAGE + L::Q, k = base + b * L::STAGE + L::K, v = base + b * L::STAGE + L::V, z = base + L::Z;
+            // (an offset of n bytes inside a tile is n >> 4 in its descriptor)
+            const uint64_t qd = tile_desc(base + b * L::STAGE + L::Q, K_MAJOR_LBO), kd = tile_desc(base + b * L::STAGE + L::K, K_MAJOR_LBO);
             if (!STATE_ONLY) {
                 ok = mbar_wait_warp(&ctl.full[b], (it >> 1) & 1, a.wait_polls);
                 if (!ok) break;
                 tc_fence_after();
                 if (lane == 0) {
+#pragma unroll
                     for (int ks = 0; ks < KB * 4; ks++) {
-                        const uint32_t at = (ks >> 2) * BLOCK_BYTES + (ks & 3) * 32;
-                        mma_ss(tmem + COL_S, tile_desc(q + at, K_MAJOR_LBO), tile_desc(k + at, K_MAJOR_LBO), idesc_s, ks > 0);
+                        const uint32_t at = ((ks >> 2) * BLOCK_BYTES + (ks & 3) * 32) >> 4;
+                        mma_ss(tmem + COL_S, qd + at, kd + at, idesc_s, ks > 0);
                     }
                     mma_commit(&ctl.s_full);
                 }
@@ -239,42 +327,162 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(DecayArgs a) {
                 if (!ok) break;
                 tc_fence_after();
                 if (lane == 0) {
+                    const uint64_t zd = tile_desc(base + L::Z, K_MAJOR_LBO);
+#pragma unroll
                     for (int ks = 0; ks < KB * 4; ks++)
-                        mma_ss(tmem + COL_QZ, tile_desc(q + (ks >> 2) * BLOCK_BYTES + (ks & 3) * 32, K_MAJOR_LBO),
-                               tile_desc(z + (ks >> 2) * (VB * 64 * 128) + (ks & 3) * 32, K_MAJOR_LBO), idesc_qz, ks > 0);
+                        mma_ss(tmem + COL_QZ, qd + (((ks >> 2) * BLOCK_BYTES + (ks & 3) * 32) >> 4),
+                               zd + (((ks >> 2) * (VB * 64 * 128) + (ks & 3) * 32) >> 4), idesc_qz, ks > 0);
                     mma_commit(&ctl.qz_full);
                 }
                 __syncwarp();
             }
             ok = mbar_wait_warp(&ctl.p_ready, it & 1, a.wait_polls);
+            // (states alone: U of the chunk before has been read)
+            if (ok && STATE_ONLY && it > 0) ok = mbar_wait_warp(&ctl.z_ready, (it - 1) & 1, a.wait_polls);
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
-                const uint32_t next = BLOCK_BYTES;  // bytes to the next 64 values
+                // along the tokens: 16 of them are 2048 bytes
+                const uint64_t vd = tile_desc(base + b * L::STAGE + L::V, BLOCK_BYTES);
+                const uint64_t vt = tile_desc(base + b * L::STAGE + L::V, VB == 2 ? BLOCK_BYTES : 0);  // (VB = 1: lanes 64 .. 127 repeat 0 .. 63)
+                const uint64_t kt = tile_desc(base + b * L::STAGE + L::K, BLOCK_BYTES), lt = tile_desc(base + b * L::STAGE + L::Q, BLOCK_BYTES);
+#pragma unroll
                 for (int ks = 0; ks < TC / 16; ks++) {
-                    const uint64_t vt = tile_desc(v + ks * 2048, VB == 2 ? next : 0);  // (VB = 1: lanes 64 .. 127 repeat 0 .. 63)
-                    mma_ss(tmem + COL_U, vt, tile_desc(k + ks * 2048, next), idesc_u, ks > 0);
-                    mma_ss(tmem + COL_U, vt, tile_desc(q + ks * 2048, next), idesc_u, 1u);
+                    mma_ss(tmem + COL_U, vt + ks * 128, kt + ks * 128, idesc_u, ks > 0);
+                    mma_ss(tmem + COL_U, vt + ks * 128, lt + ks * 128, idesc_u, 1u);
                 }
-                if (!STATE_ONLY)
+                if (!STATE_ONLY) {
+#pragma unroll
                     for (int ks = 0; ks < TC / 16; ks++)
-                        mma_f16_ts(tmem + COL_PV, tmem + COL_S + (ks >> 2) * 64 + (ks & 3) * 8, tile_desc(v + ks * 2048, next), idesc_pv, ks > 0);
+                        mma_f16_ts(tmem + COL_PV, tmem + COL_S + (ks >> 2) * 64 + (ks & 3) * 8, vd + ks * 128, idesc_pv, ks > 0);
+                }
                 mma_commit(&ctl.o_full);
                 mma_commit(&ctl.empty[b]);
             }
             __syncwarp();
             // S of the next chunk goes over P
-            ok = mbar_wait_warp(&ctl.o_full, it & 1, a.wait_polls);
+            if (!STATE_ONLY) ok = mbar_wait_warp(&ctl.o_full, it & 1, a.wait_polls);
         }
         // nothing may be in flight when tensor memory is freed
         if (lane == 0) mma_commit(&ctl.drain);
         __syncwarp();
         mbar_wait_warp(&ctl.drain, 0, TC_WAIT_POLLS);
-    } else {  // ---------------------------------------------------------------------------------- arithmetic
-        const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // lane of tensor memory, half of the columns
-        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    } else if (group == 1) {  // ------------------------------------------------------------------------ operands: P and K~
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OPERAND_REGS));
+        const int mine = tid - GROUP, r0 = (warp & 3) * 32;  // (first of the warp's rows)
+        bool ok = true;
+        for (int it = 0; it < chunks; it++) {
+            const int b = it & 1, tokens = min(TC, s.count - it * TC);
+            const int e = s.first + it * TC + tokens == s.length && !a.reverse ? tokens - 1 : tokens;
+            ok = mbar_wait_warp(&ctl.full[b], (it >> 1) & 1, a.wait_polls);
+            if (!ok) break;
+            if (tokens < TC) {  // what lies behind the chunk may be another sequence's: not even 0 * inf may come in
+                unsigned char *vt = smem + b * L::STAGE + L::V;
+                for (int p = mine; p < VB * TC * 8; p += GROUP)
+                    if (((p >> 3) & (TC - 1)) >= tokens) *reinterpret_cast<uint4 *>(vt + p * 16) = make_uint4(0, 0, 0, 0);
+            }
+            if (!STATE_ONLY) {
+                ok = mbar_wait_warp(&ctl.s_full, it & 1, a.wait_polls);
+                if (!ok) break;
+                tc_fence_after();
+                // Blocks of 32 rows x 16 columns: `side` < 0 for those before the diagonal in time (all of which count), 0 on it.
+                // (The loops of this kernel are not unrolled further than registers demand: three kinds of warps run their code
+                // at once, and unrolled it did not fit the instruction cache.)
+                float up = 1.0f;
+                if (HALF) {  // scaling from the largest of the row's products: decays only make them smaller
+                    float m = 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < 64; c += 16) {
+                        const int c0 = half * 64 + c, side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
+                        if (side > 0) continue;
+                        uint32_t r[16];
+                        tmem_ld16_nowait(lanes + COL_S + c0, r);
+                        tmem_ld_wait16(r);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) m = fmaxf(m, side < 0 || (a.reverse ? j >= d : j <= d) ? fabsf(__uint_as_float(r[j])) : 0.0f);
+                    }
+                    ctl.row_max[1][half][row] = (uint8_t)exponent_of(m);
+                    ok = meet();
+                    if (!ok) break;
+                    up = fp16_scale(max(exponent_of(m), (int)ctl.row_max[1][half ^ 1][row]));
+                    if (half == 0) ctl.p_scale[it & 1][row] = __float2bfloat16_rn(1.0f / up);
+                }
+#pragma unroll 1
+                for (int c = 0; c < 64; c += 16) {
+                    const int c0 = half * 64 + c, side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
+                    uint32_t w[8];
+                    if (side > 0) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) w[j] = 0;
+                    } else {
+                        uint32_t r[16];
+                        tmem_ld16_nowait(lanes + COL_S + c0, r);
+                        if (side < 0) {
+                            // decay = 2^(g2 (distance to the block's nearer edge)) 2^(g2 (inside the block)), both at most one
+                            const f32x2 outer = splat2(ex2_approx(g2 * (float)(a.reverse ? -d : d - 15)) * up);
+                            tmem_ld_wait16(r);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const float2 inner = *reinterpret_cast<const float2 *>(&ctl.inner[2 * j]);
+                                float u, v;
+                                unpack2(mul2(mul2(pack2(inner.x, inner.y), outer), pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))), u, v);
+                                w[j] = pack<T>(u, v);
+                            }
+                        } else {  // entry by entry
+                            const f32x2 g22 = splat2(a.reverse ? -g2 : g2), d2 = splat2((float)d), up2 = splat2(up);
+                            tmem_ld_wait16(r);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                const f32x2 x = ex2_approx2(mul2(g22, sub2(d2, pack2((float)(2 * j), (float)(2 * j + 1)))));
+                                float u, v;
+                                unpack2(mul2(HALF ? mul2(x, up2) : x, pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))), u, v);
+                                w[j] = pack<T>((a.reverse ? 2 * j >= d : 2 * j <= d) ? u : 0.0f, (a.reverse ? 2 * j + 1 >= d : 2 * j + 1 <= d) ? v : 0.0f);
+                            }
+                        }
+                    }
+                    // (16 columns of P in 8 of S, which this thread has read)
+                    tmem_st8(lanes + COL_S + half * 64 + c / 2, w);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+            }
+            // K~ over K, its low part over Q, which QZ has read by now
+            if (!STATE_ONLY) {
+                ok = mbar_wait_warp(&ctl.qz_full, it & 1, a.wait_polls);
+                if (!ok) break;
+            }
+            unsigned char *kt = smem + b * L::STAGE + L::K + mine * 16, *qt = smem + b * L::STAGE + L::Q + mine * 16;
+#pragma unroll 2
+            for (int i = 0; i < KB * 4; i++) {
+                uint4 x = *reinterpret_cast<const uint4 *>(kt + i * (GROUP * 16));
+                const int m = (mine >> 3) + 32 * (i & 3);
+                // (rows behind the last token are zero, whatever is in them)
+                if (m >= tokens) x = make_uint4(0, 0, 0, 0);
+                const f32x2 w = splat2(exp2f(g2 * (float)max(a.reverse ? m + 1 : e - m, 0)));  // decay to the chunk's end
+                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                uint32_t high[4], low[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float2 v = unpack<T>(in[j]);
+                    const f32x2 y = mul2(pack2(v.x, v.y), w);
+                    float y0, y1;
+                    unpack2(y, y0, y1);
+                    high[j] = pack<T>(y0, y1);
+                    const float2 r = unpack<T>(high[j]);
+                    unpack2(sub2(y, pack2(r.x, r.y)), y0, y1);
+                    low[j] = pack<T>(y0, y1);
+                }
+                *reinterpret_cast<uint4 *>(kt + i * (GROUP * 16)) = make_uint4(high[0], high[1], high[2], high[3]);
+                *reinterpret_cast<uint4 *>(qt + i * (GROUP * 16)) = make_uint4(low[0], low[1], low[2], low[3]);
+            }
+            fence_async_smem();
+            mbar_arrive(&ctl.p_ready);
+        }
+        if (!ok) ctl.dead = 1;
+    } else {  // ---------------------------------------------------------------------------------- results and state
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(RESULT_REGS));
         const bool state_row = row < VB * 64;
-        float z[NZ];
+        f32x2 z[NZ / 2];
         const bool first_segment = s.first == 0;
         const float *from = nullptr;
         int64_t step = 0;
@@ -289,37 +497,42 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(DecayArgs a) {
         }
         const float enter = first_segment && !a.reverse && s.length > 0 ? exp2f(g2) : 1.0f;
 #pragma unroll
-        for (int j = 0; j < NZ; j++) {
-            const int c = half * NZ + j;
-            z[j] = from != nullptr && c < a.dk ? from[c * step] * enter : 0.0f;
+        for (int j = 0; j < NZ / 2; j++) {
+            const int c = half * NZ + 2 * j;
+            z[j] = pack2(from != nullptr && c < a.dk ? from[c * step] * enter : 0.0f,
+                         from != nullptr && c + 1 < a.dk ? from[(c + 1) * step] * enter : 0.0f);
         }
-        // all arithmetic threads meet (false: gave up)
-        unsigned meetings = 0;
-        const auto meet = [&]() {
-            mbar_arrive(&ctl.meet);
-            return mbar_wait_warp(&ctl.meet, meetings++ & 1, a.wait_polls);
-        };
         // the state's copy in 16 bits for the products of chunk `it`
         const auto publish = [&](int it) {
             float f = 1.0f;
             if (HALF) {
                 float m = 0.0f;
 #pragma unroll
-                for (int j = 0; j < NZ; j++) m = fmaxf(m, fabsf(z[j]));
-                ctl.row_max[half][row] = m;
+                for (int j = 0; j < NZ / 2; j++) {
+                    float u, v;
+                    unpack2(z[j], u, v);
+                    m = fmaxf(m, fmaxf(fabsf(u), fabsf(v)));
+                }
+                ctl.row_max[0][half][row] = (uint8_t)exponent_of(m);
                 if (!meet()) return false;
-                f = fp16_scale(fmaxf(m, ctl.row_max[half ^ 1][row]));
+                f = fp16_scale(max(exponent_of(m), (int)ctl.row_max[0][half ^ 1][row]));
                 if (half == 0) ctl.z_scale[it & 1][row] = __float2bfloat16_rn(1.0f / f);
                 if (!meet()) return false;
             }
             if (!state_row) return true;
+            const f32x2 f2 = splat2(f);
 #pragma unroll
             for (int c = 0; c < NZ / 8; c++) {
                 const int chunk = half * (NZ / 8) + c;  // of 8 values, in the row
                 unsigned char *at = smem + L::Z + (chunk >> 3) * (VB * 64 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4 *>(at) =
-                    make_uint4(pack<T>(z[8 * c] * f, z[8 * c + 1] * f), pack<T>(z[8 * c + 2] * f, z[8 * c + 3] * f),
-                               pack<T>(z[8 * c + 4] * f, z[8 * c + 5] * f), pack<T>(z[8 * c + 6] * f, z[8 * c + 7] * f));
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float u, v;
+                    unpack2(HALF ? mul2(z[4 * c + j], f2) : z[4 * c + j], u, v);
+                    w[j] = pack<T>(u, v);
+                }
+                *reinterpret_cast<uint4 *>(at) = make_uint4(w[0], w[1], w[2], w[3]);
             }
             return true;
         };
@@ -329,195 +542,189 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(DecayArgs a) {
             fence_async_smem();
             mbar_arrive(&ctl.z_ready);
         }
+        // how results leave: rounds of CB columns, 16 bytes (VALUES) of a row by a lane, ROWS rows at once
+        constexpr int PER = 128 / (int)sizeof(O), CB = NO < PER ? NO : PER, VALUES = 16 / (int)sizeof(O), ACROSS = CB / VALUES, ROWS = 32 / ACROSS;
+        constexpr int PITCH = CB * (int)sizeof(O);
         const bool out_aligned = rows_aligned(a.out, sizeof(O));
+        O *const out = a.out.data == nullptr ? nullptr : a.out.at<O>(a.starts == nullptr ? s.seq : 0, hg, hi);
         const float intra = a.scale_in * a.scale_out;
+        float inter = 0.0f;  // decay of the state to this row
         int it = 0;
         for (; it < chunks && ok; it++) {
-            const int b = it & 1;
-            const int64_t first = s.first + (int64_t)it * TC;
-            const int tokens = (int)min((int64_t)TC, s.first + s.count - first);
-            const int e = first + tokens == s.length && !a.reverse ? tokens - 1 : tokens;
-            ok = mbar_wait_warp(&ctl.full[b], (it >> 1) & 1, a.wait_polls);
-            if (!ok) break;
-            float p_scale = 1.0f;  // fp16: takes the scaling of P's row back
-            if (!STATE_ONLY) {
-                ok = mbar_wait_warp(&ctl.s_full, it & 1, a.wait_polls);
-                if (!ok) break;
-                tc_fence_after();
-                float f = intra;
-                if (HALF) {  // scaling from the largest of the row's products: decays only make them smaller
-                    float m = 0.0f;
-#pragma unroll
-                    for (int cb = 0; cb < 2; cb++) {
-                        if (half * 64 + cb * 32 > (warp & 3) * 32 + 31) continue;
-                        uint32_t r[32];
-                        tmem_ld32(lanes + COL_S + half * 64 + cb * 32, r);
-                        tmem_ld_wait32(r);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) m = fmaxf(m, half * 64 + cb * 32 + j <= row ? fabsf(__uint_as_float(r[j])) : 0.0f);
-                    }
-                    ctl.row_max[half][row] = m;
-                    ok = meet();
-                    if (!ok) break;
-                    const float up = fp16_scale(fabsf(intra) * fmaxf(m, ctl.row_max[half ^ 1][row]));
-                    f *= up;
-                    p_scale = 1.0f / up;
-                }
-#pragma unroll
-                for (int cb = 0; cb < 2; cb++) {
-                    const int c0 = half * 64 + cb * 32;
-                    uint32_t w[16];
-                    if (c0 > (warp & 3) * 32 + 31) {  // all of it later than all of these rows
-#pragma unroll
-                        for (int j = 0; j < 16; j++) w[j] = 0;
-                    } else {
-                        uint32_t r[32];
-                        tmem_ld32(lanes + COL_S + c0, r);
-                        tmem_ld_wait32(r);
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            const int d = row - (c0 + 2 * j);
-                            const float x = d >= 0 ? __uint_as_float(r[2 * j]) * (f * ex2_approx(g2 * (float)d)) : 0.0f;
-                            const float y = d >= 1 ? __uint_as_float(r[2 * j + 1]) * (f * ex2_approx(g2 * (float)(d - 1))) : 0.0f;
-                            w[j] = pack<T>(x, y);
-                        }
-                    }
-                    // (columns 0 .. 31 and 64 .. 95 of S: inside what this thread alone has read)
-                    tmem_st16(lanes + COL_S + half * 64 + cb * 16, w);
-                }
-                tmem_st_wait();
-                tc_fence_before();
-                ok = mbar_wait_warp(&ctl.qz_full, it & 1, a.wait_polls);
-                if (!ok) break;
-            }
-            // K~ over K, its low part over Q
-            unsigned char *kt = smem + b * L::STAGE + L::K, *qt = smem + b * L::STAGE + L::Q;
-#pragma unroll 4
-            for (int p = tid; p < KB * TC * 8; p += COMPUTE) {
-                const int t = (p >> 3) & (TC - 1);
-                const float w = exp2f(g2 * (float)(e - t));
-                const uint4 x = *reinterpret_cast<const uint4 *>(kt + p * 16);
-                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-                uint32_t hi4[4], lo4[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float2 v = unpack<T>(in[j]);
-                    // (rows behind the last token are zero, whatever their weight)
-                    v.x = t < tokens ? v.x * w : 0.0f, v.y = t < tokens ? v.y * w : 0.0f;
-                    hi4[j] = pack<T>(v.x, v.y);
-                    const float2 r = unpack<T>(hi4[j]);
-                    lo4[j] = pack<T>(v.x - r.x, v.y - r.y);
-                }
-                *reinterpret_cast<uint4 *>(kt + p * 16) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-                *reinterpret_cast<uint4 *>(qt + p * 16) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-            }
-            fence_async_smem();
-            mbar_arrive(&ctl.p_ready);
-
+            const int b = it & 1, tokens = min(TC, s.count - it * TC);
+            const int e = s.first + it * TC + tokens == s.length && !a.reverse ? tokens - 1 : tokens;
+            const float carry = exp2f(g2 * (float)e);
+            if (it == 0 || tokens < TC) inter = exp2f(g2 * (float)(a.reverse ? tokens - 1 - row : row)) * a.scale_out;
             ok = mbar_wait_warp(&ctl.o_full, it & 1, a.wait_polls);
+            if (HALF && !STATE_ONLY) ok = ok && mbar_wait_warp(&ctl.p_ready, it & 1, a.wait_polls);  // (p_scale; long complete)
+            ok = ok && *reinterpret_cast<volatile int *>(&ctl.dead) == 0;
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const float carry = exp2f(g2 * (float)e);
+            const f32x2 carry2 = splat2(carry), in2 = splat2(a.scale_in);
 #pragma unroll
             for (int cb = 0; cb < NZ / 32; cb++) {
                 uint32_t r[32];
                 tmem_ld32(lanes + COL_U + half * NZ + cb * 32, r);
                 tmem_ld_wait32(r);
 #pragma unroll
-                for (int j = 0; j < 32; j++) z[cb * 32 + j] = fmaf(carry, z[cb * 32 + j], a.scale_in * __uint_as_float(r[j]));
-            }
-            if (!STATE_ONLY) {
-                ok = publish(it + 1);
-                if (!ok) break;
-                fence_async_smem();
-                const float f = exp2f(g2 * (float)row) * a.scale_out;
-                uint32_t out[VB][16];
-                O *to = a.out.at<O>(a.starts == nullptr ? s.seq : 0, hg, hi) + token_row(a, s, first + row) * a.out.row;
-                const bool store = row < tokens;
-#pragma unroll
-                for (int cb = 0; cb < VB; cb++) {
-                    const int c0 = half * NO + cb * 32;
-                    uint32_t x[32], y[32];
-                    tmem_ld32(lanes + COL_PV + c0, x);
-                    tmem_ld32(lanes + COL_QZ + c0, y);
-                    tmem_ld_wait32(x);
-                    tmem_ld_wait32(y);
-                    float o[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        float q = f * __uint_as_float(y[j]);
-                        if (HALF) q *= __bfloat162float(ctl.z_scale[it & 1][c0 + j]);
-                        o[j] = fmaf(p_scale, __uint_as_float(x[j]), q);
-                    }
-                    if constexpr (sizeof(O) == 2) {
-#pragma unroll
-                        for (int j = 0; j < 16; j++) out[cb][j] = pack<T>(o[2 * j], o[2 * j + 1]);
-                    } else if (store) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            if (out_aligned && c0 + j + 4 <= a.dv) {
-                                *reinterpret_cast<float4 *>(to + c0 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 4; i++)
-                                    if (c0 + j + i < a.dv) to[(c0 + j + i) * a.out.col] = o[j + i];
-                            }
-                        }
-                    }
+                for (int j = 0; j < 16; j++) {
+                    f32x2 &to = z[cb * 16 + j];
+                    to = fma2(carry2, to, mul2(in2, pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))));
                 }
+                // (done with r before the next load: registers)
+#pragma unroll
+                for (int j = 0; j < 16; j++) asm volatile("" : "+l"(z[cb * 16 + j]));
+            }
+            if (STATE_ONLY) {
                 tc_fence_before();
                 mbar_arrive(&ctl.z_ready);
-                if constexpr (sizeof(O) == 2) {
-                    if (store) {
+                continue;
+            }
+            ok = publish(it + 1);
+            if (!ok) break;
+            fence_async_smem();
+            // Results leave through the stage's Q tile (K~'s low part has been read), a warp's 32 rows of up to 128 bytes at a
+            // time, by TMA: with all of shared memory in use there is next to no L1 for stores of the threads (a chunk's results
+            // took them 3000 cycles).  The rows around a sequence's end and what has no map do take that way.
+            const float fp = HALF ? intra * __bfloat162float(ctl.p_scale[it & 1][row]) : intra;
+            unsigned char *box = smem + b * L::STAGE + L::Q + warp * 4096;
+            static_assert(L::K >= 8 * 4096, "a box for each warp");
 #pragma unroll
-                        for (int cb = 0; cb < VB; cb++)
+            for (int round = 0; round < NO / CB; round++) {
+                if (round > 0) __syncwarp();
+#pragma unroll 1
+                for (int cb = 0; cb < CB; cb += 16) {
+                    const int c0 = half * NO + round * CB + cb;
+                    uint32_t x[16], y[16];
+                    tmem_ld16_nowait(lanes + COL_PV + c0, x);
+                    tmem_ld16_nowait(lanes + COL_QZ + c0, y);
+                    tmem_ld_wait16(x);
+                    tmem_ld_wait16(y);
+                    const f32x2 fp2 = splat2(fp), inter2 = splat2(inter);
+                    uint32_t w[sizeof(O) == 2 ? 8 : 16];
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const int c = half * NO + cb * 32 + j * 8;
-                                if (out_aligned && c + 8 <= a.dv) {
-                                    *reinterpret_cast<uint4 *>(to + c) = make_uint4(out[cb][4 * j], out[cb][4 * j + 1], out[cb][4 * j + 2], out[cb][4 * j + 3]);
-                                } else {
+                    for (int j = 0; j < 8; j++) {
+                        f32x2 q = mul2(inter2, pack2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1])));
+                        if (HALF) {
+                            const float2 f = unpack<__nv_bfloat16>(*reinterpret_cast<const uint32_t *>(&ctl.z_scale[it & 1][c0 + 2 * j]));
+                            q = mul2(q, pack2(f.x, f.y));
+                        }
+                        float u, v;
+                        unpack2(fma2(fp2, pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), q), u, v);
+                        if constexpr (sizeof(O) == 2) {
+                            w[j] = pack<T>(u, v);
+                        } else {
+                            w[2 * j] = __float_as_uint(u), w[2 * j + 1] = __float_as_uint(v);
+                        }
+                    }
 #pragma unroll
-                                    for (int i = 0; i < 8; i++)
-                                        if (c + i < a.dv) {
-                                            const uint32_t w = out[cb][4 * j + i / 2];
-                                            reinterpret_cast<unsigned short *>(to)[(c + i) * a.out.col] = (unsigned short)(i & 1 ? w >> 16 : w);
-                                        }
-                                }
-                            }
+                    for (int j = 0; j < 16 / VALUES; j++)
+                        *reinterpret_cast<uint4 *>(box + swizzled<PITCH>(lane * PITCH + (cb / VALUES + j) * 16)) =
+                            make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                }
+                const int r0 = (warp & 3) * 32, x0 = half * NO + round * CB, to_row = chunk_row(a, s, it, tokens);
+                const bool by_map = maps.use[3] && r0 + 32 <= tokens;
+                if (by_map) fence_async_smem();
+                if (round == NO / CB - 1) {
+                    tc_fence_before();
+                    mbar_arrive(&ctl.z_ready);
+                }
+                __syncwarp();
+                if (by_map) {
+                    if (lane == 0 && x0 < a.dv) {
+                        tma_store(maps.out, x0, maps.by_group[3] * (int)hg + maps.by_head[3] * (int)hi, to_row + r0,
+                                  maps.by_seq[3] * (a.starts == nullptr ? s.seq : 0), box);
+                        tma_store_wait();
+                    }
+                    continue;
+                }
+                const int piece = lane % ACROSS, c = x0 + piece * VALUES, t0 = r0 + lane / ACROSS;
+                O *to = out + (int64_t)(to_row + t0) * a.out.row + c * a.out.col;
+#pragma unroll 1
+                for (int i = 0; i < 32 / ROWS; i++, to += ROWS * a.out.row) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(box + swizzled<PITCH>((i * ROWS + lane / ACROSS) * PITCH + piece * 16));
+                    if (t0 + i * ROWS >= tokens || c >= a.dv) continue;
+                    if (out_aligned && c + VALUES <= a.dv) {
+                        *reinterpret_cast<uint4 *>(to) = w;
+                    } else {
+                        O x[VALUES];
+                        memcpy(x, &w, 16);
+#pragma unroll
+                        for (int j = 0; j < VALUES; j++)
+                            if (c + j < a.dv) to[j * a.out.col] = x[j];
                     }
                 }
-            } else {
-                tc_fence_before();
             }
-        }
-        if (!ok) {  // gave up: say so, and leave nothing that looks like a result
-            ctl.dead = 1;
-#pragma unroll
-            for (int j = 0; j < NZ; j++) z[j] = __int_as_float(0x7fc00000);
-            if (!STATE_ONLY)
-                for (int64_t i = s.first + (int64_t)it * TC + row; i < s.first + s.count; i += TC) {
-                    O *to = a.out.at<O>(a.starts == nullptr ? s.seq : 0, hg, hi) + token_row(a, s, i) * a.out.row;
-                    for (int c = half * NO; c < min((half + 1) * NO, a.dv); c++) to[c * a.out.col] = from_float<O>(__int_as_float(0x7fc00000));
-                }
+            mbar_arrive(&ctl.q_empty[b]);
         }
         if (row < a.dv && (STATE_ONLY || (s.last && a.state_out.data != nullptr))) {
             float *to = STATE_ONLY ? a.states + (slot * a.heads + h) * (int64_t)a.dk * a.dv + row
                                    : a.state_out.at<float>(s.seq, hg, hi) + row * a.state_out.col;
             const int64_t row_step = STATE_ONLY ? a.dv : a.state_out.row;
 #pragma unroll
-            for (int j = 0; j < NZ; j++)
-                if (half * NZ + j < a.dk) to[(half * NZ + j) * row_step] = z[j];
+            for (int j = 0; j < NZ / 2; j++) {
+                float u, v;
+                unpack2(z[j], u, v);
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    if (half * NZ + 2 * j + i < a.dk) to[(half * NZ + 2 * j + i) * row_step] = ok ? (i ? v : u) : __int_as_float(0x7fc00000);
+            }
+        }
+        if (!ok) {  // gave up: say so, and leave nothing that looks like a result
+            ctl.dead = 1;
+            if (!STATE_ONLY)
+                poison_rows<O>(out, a.out.row, a.out.col, a.reverse ? s.begin + s.length - s.first - s.count : s.begin + s.first + it * TC,
+                               a.reverse ? s.begin + s.length - s.first - it * TC : s.begin + s.first + s.count, half * NO, min((half + 1) * NO, a.dv));
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == COMPUTE / 32) tmem_free(tmem, 512);
+    if (warp == MMA_WARP) tmem_free(tmem, 512);
     if (tid == 0 && ctl.dead != 0 && a.gave_up != nullptr) {
         *reinterpret_cast<volatile int *>(a.gave_up) = GAVE_UP_DECAY;
         __threadfence_system();
     }
+}
+
+// The map of one operand, if its rows and values allow one.
+static bool make_map(CUtensorMap *map, const DecayArgs &a, const Operand &o, int dim, CUtensorMapDataType type, int size, int width, int rows,
+                     int *by_group, int *by_head, int *by_seq) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    if (encode == nullptr || a.tokens < 1) return false;
+    if (o.col != 1 || o.row <= 0 || o.seq < 0 || o.group < 0 || o.head < 0) return false;
+    if ((reinterpret_cast<uintptr_t>(o.data) | (uintptr_t)((o.seq | o.group | o.head | o.row) * size)) & 15) return false;
+    // heads: all of them (stride o.head), one to a group (stride o.group), or one in all
+    const int64_t groups = a.heads / a.group;
+    int64_t heads = 1, head_stride = 16;
+    *by_group = *by_head = 0;
+    if (o.head != 0 && a.group > 1) {
+        if (o.group != o.head * a.group && groups > 1) return false;
+        heads = a.heads, head_stride = o.head;
+        *by_group = (int)a.group, *by_head = 1;
+    } else if (o.group != 0 && groups > 1) {
+        heads = groups, head_stride = o.group;
+        *by_group = 1;
+    }
+    const bool batch = a.starts == nullptr && a.sequences > 1 && o.seq != 0;
+    *by_seq = batch ? 1 : 0;
+    const cuuint64_t sizes[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)a.tokens, (cuuint64_t)(batch ? a.sequences : 1)};
+    const cuuint64_t strides[3] = {(cuuint64_t)(head_stride * size), (cuuint64_t)(o.row * size), (cuuint64_t)((batch ? o.seq : 16) * size)};
+    for (cuuint64_t stride : strides)
+        if (stride >= (1ull << 40)) return false;
+    const cuuint32_t box[4] = {(cuuint32_t)width, 1, (cuuint32_t)rows, 1}, ones[4] = {1, 1, 1, 1};
+    return encode(map, type, 4, o.data, sizes, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  width * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, typename O, int KB, int VB, bool STATE_ONLY>
@@ -527,7 +734,16 @@ static int launch_one(const DecayArgs &a, cudaStream_t s) {
     static_assert(bytes <= 232448, "shared memory of an SM");
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return cuda_fail(err, "decay_tc_kernel");
-    kernel<<<(unsigned)(a.slots * a.heads), THREADS, bytes, s>>>(a);
+    Maps maps = {};
+    const Operand *operands[3] = {&a.q, &a.k, &a.v};
+    CUtensorMap *map[3] = {&maps.q, &maps.k, &maps.v};
+    constexpr CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = STATE_ONLY ? 1 : 0; i < 3; i++)
+        maps.use[i] = make_map(map[i], a, *operands[i], i == 2 ? a.dv : a.dk, type, 2, 64, TC, &maps.by_group[i], &maps.by_head[i], &maps.by_seq[i]);
+    if (!STATE_ONLY)
+        maps.use[3] = make_map(&maps.out, a, a.out, a.dv, sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type, (int)sizeof(O),
+                               std::min(VB * 32, 128 / (int)sizeof(O)), 32, &maps.by_group[3], &maps.by_head[3], &maps.by_seq[3]);
+    kernel<<<(unsigned)(a.slots * a.heads), THREADS, bytes, s>>>(a, maps);
     KM_CHECK_LAUNCH("decay_tc_kernel launch");
     return KM_OK;
 }
