@@ -30,7 +30,7 @@ template <typename T, typename O, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
     extern __shared__ __align__(16) float smem[];
     float *sq = smem, *sk = sq + FC * FLD, *sv = sk + FC * FLD, *sp = sv + FC * FLD, *sz = sp + FC * 36;
-    const int64_t h = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
+    const int64_t h = blockIdx.x % (unsigned)a.heads, slot = blockIdx.x / (unsigned)a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
     const Segment s = find_segment(a, slot);
     if (!STATE_ONLY && s.spare >= 0) clear_spare_rows<O>(a, s, hg, hi);
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
 // States at the start of each segment, in place: states[slot] held the segment's own contribution.  A thread takes one
 // value of the state through the segments of a sequence, eight of them loaded ahead: read and written once.
 __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
-    const int64_t h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
+    const int64_t h = blockIdx.x % (unsigned)a.heads, seq = blockIdx.x / (unsigned)a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
     const int64_t slot0 = segments_before(a, seq);
     int64_t begin, length;
@@ -667,12 +667,18 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.scale_in = 1.0f, a.scale_out = p.scale;
     const Operand d = make_operand(dout), ds = make_operand(dstate);
-    const int vblocks = (int)ceil_div(p.dv, GV);
+    const bool tc = p.path == 2;
+    a.wait_polls = current_wait_polls();
+    a.gave_up = tc ? gave_up_word() : nullptr;
+    const int vblocks = tc ? 1 : (int)ceil_div(p.dv, GV);
     const int64_t ctas = p.sequences * a.heads * vblocks;
     KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_gradient: more than 2^31 work items");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double *partials = static_cast<double *>(workspace);
-    if (ctas > 0) {
+    if (ctas > 0 && tc) {
+        rc = launch_decay_grad_tc(p, a, d, ds, partials, s);
+        if (rc != KM_OK) return rc;
+    } else if (ctas > 0) {
         auto kernel = p.dtype == KM_TYPE_F32    ? decay_gradient_kernel<float>
                       : p.dtype == KM_TYPE_BF16 ? decay_gradient_kernel<__nv_bfloat16>
                                                 : decay_gradient_kernel<__half>;

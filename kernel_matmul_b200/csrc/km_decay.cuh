@@ -34,7 +34,8 @@ struct DecayArgs {
     Operand q, k, v, out, state_in, state_out;  // data == nullptr: absent
     const float *log_decay;
     const int32_t *starts;  // null: every sequence has `tokens` rows of its own
-    int64_t sequences, tokens, group, heads;
+    int64_t sequences, tokens;
+    unsigned group, heads;
     int dk, dv;
     int64_t segment;        // tokens of a segment (a multiple of the chunk)
     int64_t slots;          // segments of all sequences, at most
@@ -178,6 +179,8 @@ __device__ __forceinline__ void clear_spare_rows(const DecayArgs &a, const Segme
     }
 }
 
+int launch_decay_grad_tc(const km_decay_problem &p, const DecayArgs &a, const Operand &dout, const Operand &dstate, double *partials,
+                         cudaStream_t stream);
 int launch_decay_tc(const km_decay_problem &p, const DecayArgs &a, bool state_only, cudaStream_t stream);
 
 }  // namespace km

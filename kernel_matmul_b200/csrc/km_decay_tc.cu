@@ -16,32 +16,18 @@
 // Bound by memory: a chunk of a head with dk = dv = 128 moves 128 KB and takes five products of 128^3 (1300 cycles of the tensor
 // pipe), while its share of HBM takes 5600 cycles.  So everything is about keeping loads in flight: two stages of Q, K, V (96 KB
 // each), filled through TMA; K~ goes over K and Q once S and QZ have read them, P over S.
-#include <cuda.h>
-
-#include <type_traits>
-
-#include "km_decay.cuh"
+#include "km_decay_tc.cuh"
 
 namespace km {
 
 namespace {
 
-constexpr int TC = 128;       // tokens of a chunk
 constexpr int GROUP = 256;    // threads of a group: two per lane of tensor memory
 // warps 0 - 7: results and state; 8 - 15: operands; 16: matrix products; 17, 18: loads; 19: none
 constexpr int MMA_WARP = 16, THREADS = 640;
 // Registers: 640 threads are launched with 96 each, 61 440 in all, which the groups divide: 256 x 128 + 256 x 72 + 128 x 80.
 constexpr int RESULT_REGS = 144, OPERAND_REGS = 64, OTHER_REGS = 64;
 static_assert(256 * RESULT_REGS + 256 * OPERAND_REGS + 128 * OTHER_REGS <= THREADS * 96, "registers at launch");
-constexpr int BLOCK_BYTES = TC * 128;  // 128 rows of 64 values
-
-// Tiles hold rows in the order of memory, in the reverse form too, which goes through the chunks from the last: row `m` of
-// a chunk of n tokens is token m, or token n - 1 - m in the order in which the sequence is gone through.
-__device__ __forceinline__ int chunk_row(const DecayArgs &a, const Segment &s, int chunk, int tokens) {
-    const int first = s.first + chunk * TC;
-    return s.begin + (a.reverse ? s.length - first - tokens : first);
-}
-
 template <int KB, int VB>
 struct Smem {
     // (the Q tile is also where the results leave through: 8 warps' 4 KB)
@@ -64,79 +50,6 @@ struct Control {
 // tensor memory columns
 constexpr uint32_t COL_S = 0, COL_PV = 128, COL_QZ = 256, COL_U = 384;
 
-// Operand tiles, 128-byte swizzle (layout type 2).  Along the values (K-major): groups of 8 rows 1024 bytes apart.  Along the
-// tokens (MN-major): `lbo` bytes to the next 64 values, 1024 to the next 8 tokens.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t lbo) {
-    return smem_desc(addr, lbo, 1024) | (2ull << 61);
-}
-constexpr uint32_t K_MAJOR_LBO = 16;
-
-// D (+)= A B, both operands in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t"
-        "}"
-        :
-        : "r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-        "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-// The wait for the loads into `r`, tied to its registers (km_tcgen05.cuh, tmem_ld_wait16).
-__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 :
-                 : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-
-// two values as one word, the first in the low half, rounded to nearest
-template <typename T>
-__device__ __forceinline__ uint32_t pack(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return reinterpret_cast<const uint32_t &>(v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return reinterpret_cast<const uint32_t &>(v);
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack(uint32_t w);
-template <>
-__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
-    return __half22float2(reinterpret_cast<const __half2 &>(w));
-}
-
 // 2^n that brings a largest magnitude of (biased) exponent e to [2^13, 2^14) (fp16's range and as many of its small values as possible); 1 for 0 and
 // for what is not finite
 __device__ __forceinline__ int exponent_of(float m) { return (int)((__float_as_uint(m) >> 23) & 0xffu); }
@@ -152,25 +65,12 @@ __device__ __forceinline__ int swizzled(int offset) {
     return offset ^ (((offset >> 7) & (PITCH / 16 - 1)) << 4);
 }
 
-// Whether every row starts on a boundary of 16 bytes.
-__device__ __forceinline__ bool rows_aligned(const Operand &o, int size) {
-    return o.col == 1 && ((reinterpret_cast<uintptr_t>(o.data) | (uintptr_t)((o.seq | o.group | o.head | o.row) * size)) & 15) == 0;
-}
-
 // Tensor maps of q, k, v (boxes of 64 values x 128 tokens) and the result (up to 128 bytes x 32 tokens), and which operands have
 // one; the coordinates of a head and a sequence in them.
 struct Maps {
     CUtensorMap q, k, v, out;
     int use[4], by_group[4], by_head[4], by_seq[4];
 };
-
-__device__ __forceinline__ void tma_load(unsigned char *dst, const CUtensorMap &map, int x, int head, int row, int seq, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-            smem_u32(dst)),
-        "l"(&map), "r"(x), "r"(head), "r"(row), "r"(seq), "r"(smem_u32(bar))
-        : "memory");
-}
 
 __device__ __forceinline__ void tma_store(const CUtensorMap &map, int x, int head, int row, int seq, const unsigned char *src) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(&map), "r"(x), "r"(head), "r"(row),
@@ -180,24 +80,6 @@ __device__ __forceinline__ void tma_store(const CUtensorMap &map, int x, int hea
 }
 // Shared memory that this thread's stores read may be written again.
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-
-// Rows [0, tokens) of a tile without a tensor map (rows or values that do not lie on boundaries of 16 bytes), by a warp; zeros
-// behind them.  `src` is the head's value (row `first`, 0).
-template <typename T, int BLOCKS>
-__device__ __noinline__ void copy_tile(unsigned char *tile, const T *src, int64_t row, int64_t col, int tokens, int dim, int lane) {
-    constexpr int PIECES = BLOCKS * 8;
-    for (int i = lane; i < TC * PIECES; i += 32) {
-        const int r = i / PIECES, c = i % PIECES;
-        union {
-            T v[8];
-            uint4 w;
-        } x;
-        x.w = make_uint4(0, 0, 0, 0);
-        if (r < tokens)
-            for (int j = 0; j < min(dim - c * 8, 8); j++) x.v[j] = src[r * row + (c * 8 + j) * col];
-        *reinterpret_cast<uint4 *>(tile + (c >> 3) * BLOCK_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x.w;
-    }
-}
 
 // NaN into columns [c0, c1) of rows [first, end), by a warp.
 template <typename O>
@@ -218,7 +100,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     Control &ctl = *reinterpret_cast<Control *>(smem + L::REST);
 
-    const int64_t h = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
+    const int64_t h = blockIdx.x % (unsigned)a.heads, slot = blockIdx.x / (unsigned)a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
     const Segment s = find_segment(a, slot);
     if (!STATE_ONLY && s.spare >= 0) clear_spare_rows<O>(a, s, hg, hi);
@@ -354,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 if (!STATE_ONLY) {
 #pragma unroll
                     for (int ks = 0; ks < TC / 16; ks++)
-                        mma_f16_ts(tmem + COL_PV, tmem + COL_S + (ks >> 2) * 64 + (ks & 3) * 8, vd + ks * 128, idesc_pv, ks > 0);
+                        mma_f16_ts(tmem + COL_PV, tmem + COL_S + ks * 16, vd + ks * 128, idesc_pv, ks > 0);
                 }
                 mma_commit(&ctl.o_full);
                 mma_commit(&ctl.empty[b]);
@@ -392,8 +274,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 if (HALF) {  // scaling from the largest of the row's products: decays only make them smaller
                     float m = 0.0f;
 #pragma unroll 1
-                    for (int c = 0; c < 64; c += 16) {
-                        const int c0 = half * 64 + c, side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
+                    for (int c0 = half * 16; c0 < TC; c0 += 32) {
+                        const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
                         if (side > 0) continue;
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
@@ -408,8 +290,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                     if (half == 0) ctl.p_scale[it & 1][row] = __float2bfloat16_rn(1.0f / up);
                 }
 #pragma unroll 1
-                for (int c = 0; c < 64; c += 16) {
-                    const int c0 = half * 64 + c, side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
+                for (int c0 = half * 16; c0 < TC; c0 += 32) {
+                    const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
                     uint32_t w[8];
                     if (side > 0) {
 #pragma unroll
@@ -440,8 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                             }
                         }
                     }
-                    // (16 columns of P in 8 of S, which this thread has read)
-                    tmem_st8(lanes + COL_S + half * 64 + c / 2, w);
+                    tmem_st8(lanes + COL_S + c0, w);  // (over the first 8 of the 16 columns that have been read)
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -452,13 +333,13 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 if (!ok) break;
             }
             unsigned char *kt = smem + b * L::STAGE + L::K + mine * 16, *qt = smem + b * L::STAGE + L::Q + mine * 16;
-#pragma unroll 2
+#pragma unroll
             for (int i = 0; i < KB * 4; i++) {
                 uint4 x = *reinterpret_cast<const uint4 *>(kt + i * (GROUP * 16));
                 const int m = (mine >> 3) + 32 * (i & 3);
                 // (rows behind the last token are zero, whatever is in them)
                 if (m >= tokens) x = make_uint4(0, 0, 0, 0);
-                const f32x2 w = splat2(exp2f(g2 * (float)max(a.reverse ? m + 1 : e - m, 0)));  // decay to the chunk's end
+                const f32x2 w = splat2(exp2f(g2 * (float)max(a.reverse ? m : tokens - 1 - m, 0)));  // decay to the chunk's last token
                 const uint32_t in[4] = {x.x, x.y, x.z, x.w};
                 uint32_t high[4], low[4];
 #pragma unroll
@@ -561,20 +442,21 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            const f32x2 carry2 = splat2(carry), in2 = splat2(a.scale_in);
+            // (K~ is decayed to the chunk's last token, which keeps its largest entries in fp16's range; the step beyond it is taken here)
+            const f32x2 carry2 = splat2(carry), in2 = splat2(a.scale_in * exp2f(g2 * (float)(e - tokens + 1)));
 #pragma unroll
-            for (int cb = 0; cb < NZ / 32; cb++) {
-                uint32_t r[32];
-                tmem_ld32(lanes + COL_U + half * NZ + cb * 32, r);
-                tmem_ld_wait32(r);
+            for (int cb = 0; cb < NZ / 16; cb++) {
+                uint32_t r[16];
+                tmem_ld16_nowait(lanes + COL_U + half * NZ + cb * 16, r);
+                tmem_ld_wait16(r);
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    f32x2 &to = z[cb * 16 + j];
+                for (int j = 0; j < 8; j++) {
+                    f32x2 &to = z[cb * 8 + j];
                     to = fma2(carry2, to, mul2(in2, pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))));
                 }
                 // (done with r before the next load: registers)
 #pragma unroll
-                for (int j = 0; j < 16; j++) asm volatile("" : "+l"(z[cb * 16 + j]));
+                for (int j = 0; j < 8; j++) asm volatile("" : "+l"(z[cb * 8 + j]));
             }
             if (STATE_ONLY) {
                 tc_fence_before();
@@ -688,8 +570,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
     }
 }
 
-// The map of one operand, if its rows and values allow one.
-static bool make_map(CUtensorMap *map, const DecayArgs &a, const Operand &o, int dim, CUtensorMapDataType type, int size, int width, int rows,
+bool make_decay_map(CUtensorMap *map, const DecayArgs &a, const Operand &o, int dim, CUtensorMapDataType type, int size, int width, int rows,
                      int *by_group, int *by_head, int *by_seq) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -739,9 +620,9 @@ static int launch_one(const DecayArgs &a, cudaStream_t s) {
     CUtensorMap *map[3] = {&maps.q, &maps.k, &maps.v};
     constexpr CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     for (int i = STATE_ONLY ? 1 : 0; i < 3; i++)
-        maps.use[i] = make_map(map[i], a, *operands[i], i == 2 ? a.dv : a.dk, type, 2, 64, TC, &maps.by_group[i], &maps.by_head[i], &maps.by_seq[i]);
+        maps.use[i] = make_decay_map(map[i], a, *operands[i], i == 2 ? a.dv : a.dk, type, 2, 64, TC, &maps.by_group[i], &maps.by_head[i], &maps.by_seq[i]);
     if (!STATE_ONLY)
-        maps.use[3] = make_map(&maps.out, a, a.out, a.dv, sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type, (int)sizeof(O),
+        maps.use[3] = make_decay_map(&maps.out, a, a.out, a.dv, sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type, (int)sizeof(O),
                                std::min(VB * 32, 128 / (int)sizeof(O)), 32, &maps.by_group[3], &maps.by_head[3], &maps.by_seq[3]);
     kernel<<<(unsigned)(a.slots * a.heads), THREADS, bytes, s>>>(a, maps);
     KM_CHECK_LAUNCH("decay_tc_kernel launch");
