@@ -197,38 +197,43 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// States at the start of each segment, in place: states[slot] held the segment's own contribution.  A thread takes one
-// value of the state through the segments of a sequence, eight of them loaded ahead: read and written once.
+// States at the start of each segment, in place: states[slot] held the segment's own contribution.  A thread takes four
+// values of the state through the segments of a sequence, four segments loaded ahead: all is read and written once.
 __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
-    const int64_t h = blockIdx.x % (unsigned)a.heads, seq = blockIdx.x / (unsigned)a.heads;
-    const int64_t hg = h / a.group, hi = h - hg * a.group;
-    const int64_t slot0 = segments_before(a, seq);
+    const unsigned h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
+    const unsigned hg = h / a.group, hi = h - hg * a.group;
+    const int slot0 = segments_before(a, seq);
     int64_t begin, length;
     sequence_rows(a, seq, begin, length);
-    const int64_t n = min(segments_of(a, length), a.slots - slot0);
+    const int n = min(segments_of(a, length), (int)a.slots - slot0);
     if (n <= 1) return;
     const float g2 = log2_decay(a.log_decay[h]);
     const float carry = exp2f(g2 * (float)a.segment), enter = a.reverse ? 1.0f : exp2f(g2);
-    const int values = a.dk * a.dv, i = blockIdx.y * 256 + threadIdx.x;
-    if (i >= values) return;
-    float zv = 0.0f;
-    if (a.state_in.data != nullptr)
-        zv = enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col];
-    float *p = a.states + (slot0 * a.heads + h) * (int64_t)values + i;
-    const int64_t step = a.heads * (int64_t)values;
-    for (int64_t j = 0; j + 1 < n; j += 8) {
-        float own[8];
+    const int values = a.dk * a.dv, first = blockIdx.y * 1024 + threadIdx.x;
+    float z[4];
 #pragma unroll
-        for (int u = 0; u < 8; u++) own[u] = j + u + 1 < n ? p[(j + u) * step] : 0.0f;
-        // (states[j] itself is the state at its start; what is left in it by the group before has been read here)
-#pragma unroll
-        for (int u = 0; u < 8; u++) {
-            if (j + u > 0 && j + u < n) p[(j + u) * step] = zv;
-            zv = fmaf(carry, zv, own[u]);
-        }
+    for (int c = 0; c < 4; c++) {
+        const int i = first + 256 * c;
+        z[c] = a.state_in.data != nullptr && i < values
+                   ? enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col]
+                   : 0.0f;
     }
-    // (the last group may have ended right before the last segment)
-    if ((n - 1) % 8 == 0) p[(n - 1) * step] = zv;
+    float *p = a.states + ((int64_t)slot0 * a.heads + h) * values + first;
+    const int64_t step = (int64_t)a.heads * values;
+    for (int j = 0; j < n; j += 4) {
+        float own[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) own[u][c] = j + u + 1 < n && first + 256 * c < values ? p[(j + u) * step + 256 * c] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (j + u > 0 && j + u < n && first + 256 * c < values) p[(j + u) * step + 256 * c] = z[c];
+                z[c] = fmaf(carry, z[c], own[u][c]);
+            }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -624,7 +629,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.out = make_operand(out);
     a.state_out = make_operand(state_out);
-    a.segment = plan.segment;
+    a.segment = (unsigned)plan.segment;
     a.slots = plan.slots;
     a.states = static_cast<float *>(workspace);
     a.scale_in = p.reverse ? p.scale : 1.0f;
@@ -637,7 +642,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     if (plan.split) {
         rc = launch_main(p, a, plan.tc, true, s);
         if (rc != KM_OK) return rc;
-        decay_scan_kernel<<<dim3((unsigned)(p.sequences * a.heads), (unsigned)ceil_div(p.dk * p.dv, 256)), 256, 0, s>>>(a);
+        decay_scan_kernel<<<dim3((unsigned)(p.sequences * a.heads), (unsigned)ceil_div(p.dk * p.dv, 1024)), 256, 0, s>>>(a);
         KM_CHECK_LAUNCH("decay_scan_kernel launch");
     }
     return launch_main(p, a, plan.tc, false, s);

@@ -37,8 +37,8 @@ struct DecayArgs {
     int64_t sequences, tokens;
     unsigned group, heads;
     int dk, dv;
-    int64_t segment;        // tokens of a segment (a multiple of the chunk)
-    int64_t slots;          // segments of all sequences, at most
+    unsigned segment;       // tokens of a segment (a multiple of the chunk; the sums of tokens and a segment fit 32 bits)
+    int64_t slots;          // segments of all sequences, at most (less than 2^31, as all counts of this file)
     float *states;          // one (dk, dv) per (slot, head): the state a segment starts with
     float scale_in, scale_out;  // on k v^T, and on the result
     int reverse;
@@ -90,14 +90,14 @@ __device__ __forceinline__ void sequence_rows(const DecayArgs &a, int64_t i, int
     length = hi - lo;
 }
 
-__device__ __forceinline__ int64_t segments_of(const DecayArgs &a, int64_t length) {
-    return length <= a.segment ? 1 : (length + a.segment - 1) / a.segment;
+__device__ __forceinline__ int segments_of(const DecayArgs &a, int64_t length) {
+    return length <= a.segment ? 1 : (int)(((unsigned)length + (a.segment - 1u)) / a.segment);
 }
 
 // Segments of the sequences before `seq` (all lanes of a warp call it, all get the result).
-__device__ __forceinline__ int64_t segments_before(const DecayArgs &a, int64_t seq) {
-    if (a.starts == nullptr) return seq * segments_of(a, a.tokens);
-    int64_t sum = 0;
+__device__ __forceinline__ int segments_before(const DecayArgs &a, int64_t seq) {
+    if (a.starts == nullptr) return (int)seq * segments_of(a, a.tokens);
+    int sum = 0;
     for (int64_t i = threadIdx.x & 31; i < seq; i += 32) {
         int64_t begin, length;
         sequence_rows(a, i, begin, length);
@@ -112,26 +112,27 @@ __device__ __forceinline__ int64_t segments_before(const DecayArgs &a, int64_t s
 __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot) {
     Segment r = {};
     r.spare = -1;
-    int64_t index = 0;
+    int index = 0;
     if (a.starts == nullptr) {
-        const int64_t per = segments_of(a, a.tokens);
-        r.seq = (int)(slot / per);
-        index = slot - r.seq * per;
+        const int per = segments_of(a, a.tokens);
+        r.seq = (int)((unsigned)slot / (unsigned)per);
+        index = (int)slot - r.seq * per;
         r.used = true;
     } else {
         const int lane = threadIdx.x & 31;
-        int64_t before = 0;
+        int before = 0;
         for (int64_t base = 0; base < a.sequences && !r.used; base += 32) {
             const int64_t i = base + lane;
-            int64_t begin, length = 0, n = 0;
+            int64_t begin, length = 0;
+            int n = 0;
             if (i < a.sequences) {
                 sequence_rows(a, i, begin, length);
                 n = segments_of(a, length);
             }
-            int64_t upto = n;
+            int upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += v;
             }
             upto += before;
@@ -139,7 +140,7 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot
             if (hit != 0) {
                 const int who = __ffs(hit) - 1;
                 r.seq = (int)base + who;
-                index = slot - __shfl_sync(0xffffffffu, upto - n, who);
+                index = (int)slot - __shfl_sync(0xffffffffu, upto - n, who);
                 r.used = true;
             }
             before = __shfl_sync(0xffffffffu, upto, 31);
@@ -153,9 +154,9 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot
     int64_t begin, length;
     sequence_rows(a, r.seq, begin, length);
     r.begin = (int)begin, r.length = (int)length;
-    r.first = (int)(index * a.segment);
+    r.first = index * (int)a.segment;
     r.last = index == segments_of(a, length) - 1;
-    r.count = (int)min(length - r.first, a.segment);
+    r.count = min(r.length - r.first, (int)a.segment);
     // the very last slot is in use: its CTA sees to the rows of no sequence
     if (a.starts != nullptr && slot == a.slots - 1) r.spare = 0, r.spares = 1;
     return r;
