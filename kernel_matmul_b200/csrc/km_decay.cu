@@ -199,6 +199,9 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
 // ------------------------------------------------------------------------------------------------
 // States at the start of each segment, in place: states[slot] held the segment's own contribution.  A thread takes four
 // values of the state through the segments of a sequence, four segments loaded ahead: all is read and written once.
+//
+// TANGENT: of Z and, behind it, M = dZ/dg:  M <- e^{g n} (n Z + M) + own, n = tokens of a segment.
+template <bool TANGENT>
 __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
     const unsigned h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
     const unsigned hg = h / a.group, hi = h - hg * a.group;
@@ -210,27 +213,37 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
     const float g2 = log2_decay(a.log_decay[h]);
     const float carry = exp2f(g2 * (float)a.segment), enter = a.reverse ? 1.0f : exp2f(g2);
     const int values = a.dk * a.dv, first = blockIdx.y * 1024 + threadIdx.x;
-    float z[4];
+    constexpr int N = TANGENT ? 2 : 1;
+    float z[4], m[4];
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         const int i = first + 256 * c;
-        z[c] = a.state_in.data != nullptr && i < values
-                   ? enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col]
-                   : 0.0f;
+        z[c] = m[c] = a.state_in.data != nullptr && i < values
+                          ? enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col]
+                          : 0.0f;
     }
-    float *p = a.states + ((int64_t)slot0 * a.heads + h) * values + first;
-    const int64_t step = (int64_t)a.heads * values;
+    float *p = a.states + ((int64_t)slot0 * a.heads + h) * N * values + first;
+    const int64_t step = (int64_t)a.heads * N * values;
+    const float tokens = (float)a.segment;
     for (int j = 0; j < n; j += 4) {
-        float own[4][4];
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) own[u][c] = j + u + 1 < n && first + 256 * c < values ? p[(j + u) * step + 256 * c] : 0.0f;
+        float own[4][4], own_m[4][4];
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                if (j + u > 0 && j + u < n && first + 256 * c < values) p[(j + u) * step + 256 * c] = z[c];
+                const bool there = j + u + 1 < n && first + 256 * c < values;
+                own[u][c] = there ? p[(j + u) * step + 256 * c] : 0.0f;
+                own_m[u][c] = TANGENT && there ? p[(j + u) * step + values + 256 * c] : 0.0f;
+            }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (j + u > 0 && j + u < n && first + 256 * c < values) {
+                    p[(j + u) * step + 256 * c] = z[c];
+                    if (TANGENT) p[(j + u) * step + values + 256 * c] = m[c];
+                }
+                if (TANGENT) m[c] = fmaf(carry, fmaf(tokens, z[c], m[c]), own_m[u][c]);
                 z[c] = fmaf(carry, z[c], own[u][c]);
             }
     }
@@ -569,6 +582,13 @@ static km_decay_problem resolved(const km_decay_problem &p) {
     return r;
 }
 
+template <bool TANGENT>
+static int launch_scan(const DecayArgs &a, cudaStream_t s) {
+    decay_scan_kernel<TANGENT><<<dim3((unsigned)(a.sequences * a.heads), (unsigned)ceil_div(a.dk * a.dv, 1024)), 256, 0, s>>>(a);
+    KM_CHECK_LAUNCH("decay_scan_kernel launch");
+    return KM_OK;
+}
+
 template <typename T, typename O>
 static int launch_fma(const DecayArgs &a, bool state_only, cudaStream_t s) {
     auto kernel = state_only ? decay_fma_kernel<T, O, true> : decay_fma_kernel<T, O, false>;
@@ -642,18 +662,34 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     if (plan.split) {
         rc = launch_main(p, a, plan.tc, true, s);
         if (rc != KM_OK) return rc;
-        decay_scan_kernel<<<dim3((unsigned)(p.sequences * a.heads), (unsigned)ceil_div(p.dk * p.dv, 1024)), 256, 0, s>>>(a);
-        KM_CHECK_LAUNCH("decay_scan_kernel launch");
+        rc = launch_scan<false>(a, s);
+        if (rc != KM_OK) return rc;
     }
     return launch_main(p, a, plan.tc, false, s);
 }
+
+namespace km {
+
+// Partial sums, and values of states, of the gradient of the decays.  The kernel on the FMA pipe does not cut sequences:
+// its columns of v are independent, four CTAs to a head.
+static size_t grad_sums(const km_decay_problem &p) {
+    const size_t heads = (size_t)(p.groups * p.group);
+    return heads * (p.path == 2 ? (size_t)plan_of(p).slots : (size_t)p.sequences * (size_t)ceil_div(p.dv, GV));
+}
+static size_t grad_states(const km_decay_problem &p) {
+    if (p.path != 2) return 0;
+    const DecayPlan plan = plan_of(p);
+    return plan.split ? (size_t)plan.slots * (size_t)(p.groups * p.group * p.dk * p.dv) * 2 : 0;
+}
+
+}  // namespace km
 
 extern "C" size_t km_decay_gradient_workspace_bytes(const km_decay_problem *problem) {
     using namespace km;
     if (problem == nullptr) return 0;
     const km_decay_problem p = resolved(*problem);
     if (check_problem("km_decay_gradient_workspace_bytes", &p) != KM_OK) return 0;
-    return (size_t)(p.sequences * p.groups * p.group) * (size_t)ceil_div(p.dv, GV) * sizeof(double);
+    return grad_sums(p) * sizeof(double) + grad_states(p) * sizeof(float);
 }
 
 extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view *q, const km_view *k, const km_view *v, const km_view *dout,
@@ -675,13 +711,22 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
     const bool tc = p.path == 2;
     a.wait_polls = current_wait_polls();
     a.gave_up = tc ? gave_up_word() : nullptr;
-    const int vblocks = tc ? 1 : (int)ceil_div(p.dv, GV);
-    const int64_t ctas = p.sequences * a.heads * vblocks;
+    const DecayPlan plan = plan_of(p);
+    const int vblocks = (int)ceil_div(p.dv, GV);
+    const int64_t sums = (int64_t)grad_sums(p) / a.heads, ctas = sums * a.heads;
     KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_gradient: more than 2^31 work items");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double *partials = static_cast<double *>(workspace);
     if (ctas > 0 && tc) {
-        rc = launch_decay_grad_tc(p, a, d, ds, partials, s);
+        a.segment = (unsigned)plan.segment;
+        a.slots = plan.slots;
+        a.states = reinterpret_cast<float *>(partials + ctas);
+        if (plan.split) {
+            rc = launch_decay_grad_tc(p, a, d, ds, partials, true, s);
+            if (rc == KM_OK) rc = launch_scan<true>(a, s);
+            if (rc != KM_OK) return rc;
+        }
+        rc = launch_decay_grad_tc(p, a, d, ds, partials, false, s);
         if (rc != KM_OK) return rc;
     } else if (ctas > 0) {
         auto kernel = p.dtype == KM_TYPE_F32    ? decay_gradient_kernel<float>
@@ -692,7 +737,7 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
         kernel<<<(unsigned)ctas, 256, GRAD_SMEM, s>>>(a, d, ds, vblocks, partials);
         KM_CHECK_LAUNCH("decay_gradient_kernel launch");
     }
-    decay_gradient_finish_kernel<<<(unsigned)a.heads, 256, 0, s>>>(p.sequences * vblocks, partials, grad);
+    decay_gradient_finish_kernel<<<a.heads, 256, 0, s>>>(sums, partials, grad);
     KM_CHECK_LAUNCH("decay_gradient_finish_kernel launch");
     return KM_OK;
 }

@@ -39,7 +39,7 @@ struct DecayArgs {
     int dk, dv;
     unsigned segment;       // tokens of a segment (a multiple of the chunk; the sums of tokens and a segment fit 32 bits)
     int64_t slots;          // segments of all sequences, at most (less than 2^31, as all counts of this file)
-    float *states;          // one (dk, dv) per (slot, head): the state a segment starts with
+    float *states;          // one (dk, dv) per (slot, head): the state a segment starts with (gradient of the decays: two, Z and M)
     float scale_in, scale_out;  // on k v^T, and on the result
     int reverse;
     int *gave_up;
@@ -181,7 +181,7 @@ __device__ __forceinline__ void clear_spare_rows(const DecayArgs &a, const Segme
 }
 
 int launch_decay_grad_tc(const km_decay_problem &p, const DecayArgs &a, const Operand &dout, const Operand &dstate, double *partials,
-                         cudaStream_t stream);
+                         bool state_only, cudaStream_t stream);
 int launch_decay_tc(const km_decay_problem &p, const DecayArgs &a, bool state_only, cudaStream_t stream);
 
 }  // namespace km

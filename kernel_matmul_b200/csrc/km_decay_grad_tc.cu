@@ -16,7 +16,7 @@ namespace km {
 
 namespace {
 
-constexpr int GRAD_THREADS = 288;
+constexpr int ARITH = 512, GRAD_THREADS = ARITH + 32;  // threads of arithmetic: four per lane of tensor memory; a warp of loads and products
 constexpr float PART = 1.0f / 128.0f;  // K' and Q' are weighted with 128ths of their distances: at most one, as fp16 needs it
 constexpr uint32_t COL_S = 0, COL_G = 128, COL_U = 256, COL_U1 = 384;  // X' over S, X over G
 
@@ -30,7 +30,7 @@ struct GradControl {
     uint32_t tmem;
     int dead;
     float inner[16];  // 2^(g2 (15 - j))
-    double sums[8];
+    double sums[ARITH / 32];
 };
 
 template <int KB, int VB>
@@ -67,40 +67,40 @@ __device__ __forceinline__ void decayed_parts(uint4 x, float w, float more, uint
 
 }  // namespace
 
-template <typename T, int KB, int VB>
+// STATE_ONLY: the states that a segment adds, from zero (before decay_scan_kernel).
+template <typename T, int KB, int VB, bool STATE_ONLY>
 __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __grid_constant__ DecayArgs a, const __grid_constant__ Operand dout,
                                                                         const __grid_constant__ Operand dstate,
                                                                         const __grid_constant__ GradMaps maps, double *partials) {
     using L = GradSmem<KB, VB>;
-    constexpr int NZ = KB * 32;
+    constexpr int NZ = KB * 16;  // of the states' rows: this thread's columns
     constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
     extern __shared__ unsigned char raw[];
     unsigned char *smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     GradControl &ctl = *reinterpret_cast<GradControl *>(smem + L::CONTROL);
-    const int64_t h = blockIdx.x % (unsigned)a.heads, seq = blockIdx.x / (unsigned)a.heads;
+    const int64_t h = blockIdx.x % a.heads, slot = blockIdx.x / a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
-    Segment s = {};
-    {
-        int64_t begin, length;
-        sequence_rows(a, seq, begin, length);
-        s.seq = (int)seq, s.begin = (int)begin, s.length = s.count = (int)length;
+    const Segment s = find_segment(a, slot);
+    if (!s.used || (STATE_ONLY && s.last)) {
+        if (!STATE_ONLY && threadIdx.x == 0) partials[h * a.slots + slot] = 0.0;
+        return;
     }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = (s.count + TC - 1) / TC;
     const float g2 = log2_decay(a.log_decay[h]);
     if (tid == 0) {
         mbar_init(&ctl.full, 33), mbar_init(&ctl.sg_full, 1), mbar_init(&ctl.u_full, 1), mbar_init(&ctl.x_full, 1), mbar_init(&ctl.drain, 1);
-        mbar_init(&ctl.k_ready, 256), mbar_init(&ctl.q_ready, 256), mbar_init(&ctl.read, 256);
+        mbar_init(&ctl.k_ready, ARITH), mbar_init(&ctl.q_ready, ARITH), mbar_init(&ctl.read, ARITH);
         ctl.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc(&ctl.tmem, 512);
+    if (warp == ARITH / 32) tmem_alloc(&ctl.tmem, 512);
     if (tid < 16) ctl.inner[tid] = exp2f(g2 * (float)(15 - tid));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem, base = smem_u32(smem);
 
-    if (warp == 8) {  // ------------------------------------------------------------------------------- loads and products
+    if (warp == ARITH / 32) {  // ------------------------------------------------------------------------------- loads and products
         constexpr uint32_t idesc0 = (1u << 4) | (type << 7) | (type << 10) | ((128u >> 4) << 24);
         constexpr uint32_t idesc_sg = idesc0 | ((128u >> 3) << 17);
         constexpr uint32_t idesc_u = idesc0 | ((uint32_t)(KB * 64 >> 3) << 17) | (1u << 15) | (1u << 16);
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
         const int rows_seq = a.starts == nullptr ? s.seq : 0;
         unsigned bytes = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) bytes += maps.use[i] ? (i < 2 ? KB : VB) * BLOCK_BYTES : 0;
+        for (int i = 0; i < 4; i++) bytes += maps.use[i] && !(STATE_ONLY && (i == 0 || i == 3)) ? (i < 2 ? KB : VB) * BLOCK_BYTES : 0;
         // sum over the tokens of A^T B: A (values on the lanes) and B's parts as they lie in memory
         const auto outer = [&](uint32_t col, uint32_t a_at, uint32_t high, uint32_t low) {
             const uint64_t at = tile_desc(base + a_at, VB == 2 ? NEXT : 0), ht = tile_desc(base + high, NEXT), lt = tile_desc(base + low, NEXT);
@@ -142,17 +142,17 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                     copy_tile<T, BLOCKS>(smem + at, o.at<const T>(rows_seq, hg, hi) + (int64_t)row0 * o.row, o.row, o.col, tokens, dim, lane);
                 }
             };
-            fetch(std::integral_constant<int, KB>(), 0, a.q, L::Q, a.dk);
+            if (!STATE_ONLY) fetch(std::integral_constant<int, KB>(), 0, a.q, L::Q, a.dk);
             fetch(std::integral_constant<int, KB>(), 1, a.k, L::K, a.dk);
             fetch(std::integral_constant<int, VB>(), 2, a.v, L::V, a.dv);
-            fetch(std::integral_constant<int, VB>(), 3, dout, L::D, a.dv);
+            if (!STATE_ONLY) fetch(std::integral_constant<int, VB>(), 3, dout, L::D, a.dv);
             fence_async_smem();
             mbar_arrive(&ctl.full);
             filled++;
             ok = mbar_wait_warp(&ctl.full, it & 1, a.wait_polls) && (it == 0 || mbar_wait_warp(&ctl.read, (it - 1) & 1, a.wait_polls));
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
+            if (lane == 0 && !STATE_ONLY) {
                 inner(COL_S, L::Q, L::K, KB);
                 inner(COL_G, L::D, L::V, VB);
                 mma_commit(&ctl.sg_full);
@@ -167,6 +167,10 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                 mma_commit(&ctl.u_full);
             }
             __syncwarp();
+            if (STATE_ONLY) {
+                ok = mbar_wait_warp(&ctl.u_full, it & 1, a.wait_polls);
+                continue;
+            }
             ok = mbar_wait_warp(&ctl.q_ready, it & 1, a.wait_polls);
             if (!ok) break;
             tc_fence_after();
@@ -185,65 +189,47 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
         __syncwarp();
         mbar_wait_warp(&ctl.drain, 0, TC_WAIT_POLLS);
     } else {  // ---------------------------------------------------------------------------------------- arithmetic
-        const int row = (warp & 3) * 32 + lane, half = warp >> 2, r0 = (warp & 3) * 32;
+        const int row = (warp & 3) * 32 + lane, part = warp >> 2, r0 = (warp & 3) * 32;
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
         const bool state_row = row < VB * 64;
+        const int64_t state = (int64_t)a.dk * a.dv;
+        float *own = a.states + (slot * a.heads + h) * 2 * state;  // Z, then M (where sequences are cut)
         f32x2 z[NZ / 2], m[NZ / 2];
         {
-            const float *from = a.state_in.data != nullptr && row < a.dv ? a.state_in.at<const float>(s.seq, hg, hi) + row * a.state_in.col : nullptr;
-            const float enter = exp2f(g2);
+            const float *from = nullptr, *from_m = nullptr;
+            int64_t step = 0;
+            float enter = 1.0f;
+            if (!STATE_ONLY && row < a.dv) {
+                if (s.first > 0) {
+                    from = own + row, from_m = from + state, step = a.dv;
+                } else if (a.state_in.data != nullptr) {
+                    from = from_m = a.state_in.at<const float>(s.seq, hg, hi) + row * a.state_in.col;
+                    step = a.state_in.row, enter = exp2f(g2);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < NZ / 2; j++) {
-                const int c = half * NZ + 2 * j;
-                z[j] = m[j] = pack2(from != nullptr && c < a.dk ? from[c * a.state_in.row] * enter : 0.0f,
-                                    from != nullptr && c + 1 < a.dk ? from[(c + 1) * a.state_in.row] * enter : 0.0f);
+                const int c = part * NZ + 2 * j;
+                const bool one = from != nullptr && c < a.dk, two = from != nullptr && c + 1 < a.dk;
+                z[j] = pack2(one ? from[c * step] * enter : 0.0f, two ? from[(c + 1) * step] * enter : 0.0f);
+                m[j] = pack2(one ? from_m[c * step] * enter : 0.0f, two ? from_m[(c + 1) * step] * enter : 0.0f);
             }
         }
         double total = 0.0;
         bool ok = true;
         for (int it = 0; it < chunks; it++) {
             const int tokens = min(TC, s.count - it * TC);
-            const int e = it == chunks - 1 ? tokens - 1 : tokens;
+            const int e = s.first + it * TC + tokens == s.length ? tokens - 1 : tokens;
             const int last = tokens - 1;  // decays are relative to the chunk's last token, the step beyond it is taken in fp32
-            ok = mbar_wait_warp(&ctl.full, it & 1, a.wait_polls) && mbar_wait_warp(&ctl.sg_full, it & 1, a.wait_polls);
+            ok = mbar_wait_warp(&ctl.full, it & 1, a.wait_polls);
+            if (!STATE_ONLY) ok = ok && mbar_wait_warp(&ctl.sg_full, it & 1, a.wait_polls);
             if (!ok) break;
             tc_fence_after();
-            f32x2 sum = splat2(0.0f);
-#pragma unroll 1
-            for (int c0 = half * 16; c0 <= r0 + 31; c0 += 32) {
-                uint32_t x[16], y[16];
-                tmem_ld16_nowait(lanes + COL_S + c0, x);
-                tmem_ld16_nowait(lanes + COL_G + c0, y);
-                const int d = row - c0;
-                const bool diagonal = c0 + 31 >= r0 + 16;  // (blocks of 16 columns that reach the diagonal of the warp's rows)
-                const f32x2 outer = splat2(ex2_approx(g2 * (float)max(d - 15, 0)));
-                tmem_ld_wait16(x);
-                tmem_ld_wait16(y);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const f32x2 dist = sub2(splat2((float)d), pack2((float)(2 * j), (float)(2 * j + 1)));
-                    f32x2 w;
-                    if (diagonal) {
-                        w = ex2_approx2(mul2(splat2(g2), dist));
-                    } else {
-                        const float2 inside = *reinterpret_cast<const float2 *>(&ctl.inner[2 * j]);
-                        w = mul2(outer, pack2(inside.x, inside.y));
-                    }
-                    f32x2 v = mul2(mul2(dist, w), mul2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])),
-                                                       pack2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]))));
-                    if (diagonal || tokens < TC) {  // what is behind the diagonal or the last token may be anything
-                        float u0, u1;
-                        unpack2(v, u0, u1);
-                        v = pack2(2 * j < d && row < tokens ? u0 : 0.0f, 2 * j + 1 < d && row < tokens ? u1 : 0.0f);
-                    }
-                    sum = add2(sum, v);
-                }
-            }
             if (tokens < TC)  // rows behind the chunk may be another sequence's: not even 0 * inf may come in
-                for (int p = tid; p < 2 * VB * TC * 8; p += 256)
+                for (int p = tid; p < (STATE_ONLY ? 1 : 2) * VB * TC * 8; p += ARITH)
                     if (((p >> 3) & (TC - 1)) >= tokens) *reinterpret_cast<uint4 *>(smem + L::V + p * 16) = make_uint4(0, 0, 0, 0);
 #pragma unroll 2
-            for (int p = tid; p < KB * TC * 8; p += 256) {
+            for (int p = tid; p < KB * TC * 8; p += ARITH) {
                 const int t = (p >> 3) & (TC - 1);
                 uint4 x = *reinterpret_cast<const uint4 *>(smem + L::K + p * 16), out[4];
                 if (t >= tokens) x = make_uint4(0, 0, 0, 0);
@@ -253,43 +239,82 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                 for (int i = 0; i < 3; i++) *reinterpret_cast<uint4 *>(smem + L::SPARE + i * KB * BLOCK_BYTES + p * 16) = out[i + 1];
             }
             fence_async_smem();
-            tc_fence_before();
             mbar_arrive(&ctl.k_ready);
+            // (under the products U)
+            f32x2 sum = splat2(0.0f);
+            if (!STATE_ONLY) {
+#pragma unroll 1
+                for (int c0 = part * 16; c0 <= r0 + 31; c0 += 64) {
+                    uint32_t x[16], y[16];
+                    tmem_ld16_nowait(lanes + COL_S + c0, x);
+                    tmem_ld16_nowait(lanes + COL_G + c0, y);
+                    const int d = row - c0;
+                    const bool diagonal = c0 + 31 >= r0 + 16;  // (blocks of 16 columns that reach the diagonal of the warp's rows)
+                    const f32x2 outer = splat2(ex2_approx(g2 * (float)max(d - 15, 0)));
+                    tmem_ld_wait16(x);
+                    tmem_ld_wait16(y);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const f32x2 dist = sub2(splat2((float)d), pack2((float)(2 * j), (float)(2 * j + 1)));
+                        f32x2 w;
+                        if (diagonal) {
+                            w = ex2_approx2(mul2(splat2(g2), dist));
+                        } else {
+                            const float2 inside = *reinterpret_cast<const float2 *>(&ctl.inner[2 * j]);
+                            w = mul2(outer, pack2(inside.x, inside.y));
+                        }
+                        f32x2 v = mul2(mul2(dist, w), mul2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])),
+                                                           pack2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]))));
+                        if (diagonal || tokens < TC) {  // what is behind the diagonal or the last token may be anything
+                            float u0, u1;
+                            unpack2(v, u0, u1);
+                            v = pack2(2 * j < d && row < tokens ? u0 : 0.0f, 2 * j + 1 < d && row < tokens ? u1 : 0.0f);
+                        }
+                        sum = add2(sum, v);
+                    }
+                }
+            }
+            tc_fence_before();  // (S and G have been read before X goes over them)
             ok = mbar_wait_warp(&ctl.u_full, it & 1, a.wait_polls);
             if (!ok) break;
+            if (!STATE_ONLY) {
 #pragma unroll 2
-            for (int p = tid; p < KB * TC * 8; p += 256) {
-                const int t = (p >> 3) & (TC - 1);
-                uint4 x = *reinterpret_cast<const uint4 *>(smem + L::Q + p * 16), out[4];
-                if (t >= tokens) x = make_uint4(0, 0, 0, 0);
-                decayed_parts<T>(x, exp2f(g2 * (float)t), (float)t * PART, out);
-                *reinterpret_cast<uint4 *>(smem + L::Q + p * 16) = out[0];
+                for (int p = tid; p < KB * TC * 8; p += ARITH) {
+                    const int t = (p >> 3) & (TC - 1);
+                    uint4 x = *reinterpret_cast<const uint4 *>(smem + L::Q + p * 16), out[4];
+                    if (t >= tokens) x = make_uint4(0, 0, 0, 0);
+                    decayed_parts<T>(x, exp2f(g2 * (float)t), (float)t * PART, out);
+                    *reinterpret_cast<uint4 *>(smem + L::Q + p * 16) = out[0];
 #pragma unroll
-                for (int i = 0; i < 3; i++) *reinterpret_cast<uint4 *>(smem + L::SPARE + i * KB * BLOCK_BYTES + p * 16) = out[i + 1];
+                    for (int i = 0; i < 3; i++) *reinterpret_cast<uint4 *>(smem + L::SPARE + i * KB * BLOCK_BYTES + p * 16) = out[i + 1];
+                }
+                fence_async_smem();
+                mbar_arrive(&ctl.q_ready);
+                ok = mbar_wait_warp(&ctl.x_full, it & 1, a.wait_polls);
+                if (!ok) break;
             }
-            fence_async_smem();
-            mbar_arrive(&ctl.q_ready);
-            ok = mbar_wait_warp(&ctl.x_full, it & 1, a.wait_polls);
-            if (!ok) break;
             tc_fence_after();
             const f32x2 carry = splat2(exp2f(g2 * (float)e)), steps = splat2((float)e), whole = splat2(1.0f / PART);
             const f32x2 beyond = splat2(exp2f(g2 * (float)(e - last)));
 #pragma unroll
             for (int c = 0; c < NZ; c += 8) {
                 uint32_t x[8], x1[8], u[8], u1[8];
-                tmem_ld8_nowait(lanes + COL_G + half * NZ + c, x);
-                tmem_ld8_nowait(lanes + COL_S + half * NZ + c, x1);
-                tmem_ld8_nowait(lanes + COL_U + half * NZ + c, u);
-                tmem_ld8_nowait(lanes + COL_U1 + half * NZ + c, u1);
-                tmem_ld_wait8x2(x, x1);
+                if (!STATE_ONLY) {
+                    tmem_ld8_nowait(lanes + COL_G + part * NZ + c, x);
+                    tmem_ld8_nowait(lanes + COL_S + part * NZ + c, x1);
+                }
+                tmem_ld8_nowait(lanes + COL_U + part * NZ + c, u);
+                tmem_ld8_nowait(lanes + COL_U1 + part * NZ + c, u1);
+                if (!STATE_ONLY) tmem_ld_wait8x2(x, x1);
                 tmem_ld_wait8x2(u, u1);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     f32x2 &zz = z[c / 2 + j], &mm = m[c / 2 + j];
                     const auto pair = [](const uint32_t &p, const uint32_t &q) { return pack2(__uint_as_float(p), __uint_as_float(q)); };
-                    f32x2 v = mul2(pair(x[2 * j], x[2 * j + 1]), mm);
-                    v = fma2(mul2(whole, pair(x1[2 * j], x1[2 * j + 1])), zz, v);
-                    if (state_row) sum = add2(sum, v);  // (VB = 1: the other lanes repeat these)
+                    if (!STATE_ONLY && state_row) {  // (VB = 1: the other lanes repeat these)
+                        sum = fma2(pair(x[2 * j], x[2 * j + 1]), mm, sum);
+                        sum = fma2(mul2(whole, pair(x1[2 * j], x1[2 * j + 1])), zz, sum);
+                    }
                     mm = fma2(carry, fma2(steps, zz, mm), mul2(beyond, mul2(whole, pair(u1[2 * j], u1[2 * j + 1]))));
                     zz = fma2(carry, zz, mul2(beyond, pair(u[2 * j], u[2 * j + 1])));
                 }
@@ -304,15 +329,25 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             total += (double)(u + v);
         }
         total *= (double)a.scale_out;
-        if (dstate.data != nullptr && s.length > 0 && row < a.dv) {
+        if (!STATE_ONLY && dstate.data != nullptr && s.last && s.length > 0 && row < a.dv) {
             const float *from = dstate.at<const float>(s.seq, hg, hi) + row * dstate.col;
 #pragma unroll
             for (int j = 0; j < NZ / 2; j++) {
                 float u, v;
                 unpack2(m[j], u, v);
-                const int c = half * NZ + 2 * j;
+                const int c = part * NZ + 2 * j;
                 if (c < a.dk) total += (double)u * (double)from[c * dstate.row];
                 if (c + 1 < a.dk) total += (double)v * (double)from[(c + 1) * dstate.row];
+            }
+        }
+        if (STATE_ONLY && row < a.dv) {
+#pragma unroll
+            for (int j = 0; j < NZ / 2; j++) {
+                float u, v, u1, v1;
+                unpack2(z[j], u, v), unpack2(m[j], u1, v1);
+                const int c = part * NZ + 2 * j;
+                if (c < a.dk) own[c * a.dv + row] = u, own[state + c * a.dv + row] = u1;
+                if (c + 1 < a.dk) own[(c + 1) * a.dv + row] = v, own[state + (c + 1) * a.dv + row] = v1;
             }
         }
         if (!ok) {  // gave up: say so, and leave nothing that looks like a result
@@ -326,11 +361,11 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) tmem_free(tmem, 512);
+    if (warp == ARITH / 32) tmem_free(tmem, 512);
     if (tid == 0) {
         double v = 0.0;
-        for (int w = 0; w < 8; w++) v += ctl.sums[w];
-        partials[h * a.sequences + seq] = v;
+        for (int w = 0; w < ARITH / 32; w++) v += ctl.sums[w];
+        if (!STATE_ONLY) partials[h * a.slots + slot] = v;
         if (ctl.dead != 0 && a.gave_up != nullptr) {
             *reinterpret_cast<volatile int *>(a.gave_up) = GAVE_UP_DECAY;
             __threadfence_system();
@@ -338,32 +373,36 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
     }
 }
 
-template <typename T, int KB, int VB>
+template <typename T, int KB, int VB, bool STATE_ONLY>
 static int launch_grad(const DecayArgs &a, const Operand &dout, const Operand &dstate, double *partials, cudaStream_t s) {
-    auto kernel = decay_grad_tc_kernel<T, KB, VB>;
+    auto kernel = decay_grad_tc_kernel<T, KB, VB, STATE_ONLY>;
     constexpr int bytes = GradSmem<KB, VB>::BYTES;
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return cuda_fail(err, "decay_grad_tc_kernel");
     GradMaps maps = {};
     const Operand *operands[4] = {&a.q, &a.k, &a.v, &dout};
     constexpr CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    for (int i = 0; i < 4; i++)
+    for (int i = STATE_ONLY ? 1 : 0; i < (STATE_ONLY ? 3 : 4); i++)
         maps.use[i] = make_decay_map(&maps.map[i], a, *operands[i], i < 2 ? a.dk : a.dv, type, 2, 64, TC, &maps.by_group[i], &maps.by_head[i],
                                      &maps.by_seq[i]);
-    kernel<<<(unsigned)(a.sequences * a.heads), GRAD_THREADS, bytes, s>>>(a, dout, dstate, maps, partials);
+    kernel<<<(unsigned)(a.slots * a.heads), GRAD_THREADS, bytes, s>>>(a, dout, dstate, maps, partials);
     KM_CHECK_LAUNCH("decay_grad_tc_kernel launch");
     return KM_OK;
 }
 
-template <typename T>
+template <typename T, bool STATE_ONLY>
 static int launch_grad_dims(const DecayArgs &a, const Operand &dout, const Operand &dstate, double *partials, cudaStream_t s) {
-    if (a.dk <= 64) return a.dv <= 64 ? launch_grad<T, 1, 1>(a, dout, dstate, partials, s) : launch_grad<T, 1, 2>(a, dout, dstate, partials, s);
-    return a.dv <= 64 ? launch_grad<T, 2, 1>(a, dout, dstate, partials, s) : launch_grad<T, 2, 2>(a, dout, dstate, partials, s);
+    if (a.dk <= 64)
+        return a.dv <= 64 ? launch_grad<T, 1, 1, STATE_ONLY>(a, dout, dstate, partials, s) : launch_grad<T, 1, 2, STATE_ONLY>(a, dout, dstate, partials, s);
+    return a.dv <= 64 ? launch_grad<T, 2, 1, STATE_ONLY>(a, dout, dstate, partials, s) : launch_grad<T, 2, 2, STATE_ONLY>(a, dout, dstate, partials, s);
 }
 
 int launch_decay_grad_tc(const km_decay_problem &p, const DecayArgs &a, const Operand &dout, const Operand &dstate, double *partials,
-                         cudaStream_t s) {
-    return p.dtype == KM_TYPE_BF16 ? launch_grad_dims<__nv_bfloat16>(a, dout, dstate, partials, s) : launch_grad_dims<__half>(a, dout, dstate, partials, s);
+                         bool state_only, cudaStream_t s) {
+    if (p.dtype == KM_TYPE_BF16)
+        return state_only ? launch_grad_dims<__nv_bfloat16, true>(a, dout, dstate, partials, s)
+                          : launch_grad_dims<__nv_bfloat16, false>(a, dout, dstate, partials, s);
+    return state_only ? launch_grad_dims<__half, true>(a, dout, dstate, partials, s) : launch_grad_dims<__half, false>(a, dout, dstate, partials, s);
 }
 
 }  // namespace km
