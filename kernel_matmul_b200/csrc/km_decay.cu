@@ -255,48 +255,55 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
 //   M <- e^{g e} (e Z + M) + sum_s (e - s) e^{g (e - s)} k_s v_s^T,
 // and grad = sum_t dout_t . d out_t + <dstate, dM of the last state>: a sum of terms that are each as small as their
 // distances, where differences of sums over tokens (t q.dq - s k.dk) would cancel to a part of 1 / tokens.
-// One CTA per (sequence, head, 32 columns of v): the states' columns are independent.  All in fp32, sums over chunks in fp64.
+// One CTA per (segment, head, 32 columns of v): the states' columns are independent.  All in fp32, sums over chunks in fp64.
+// STATE_ONLY: the states that a segment adds, from zero (before the scan).
 constexpr int GV = 32;  // columns of v
 constexpr int GRAD_SMEM = (2 * FC * FLD + 2 * FC * 36 + FC * 36 + 2 * KM_DECAY_MAX_DIM * 36) * 4;
 
-template <typename T>
+template <typename T, bool STATE_ONLY>
 __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operand dout, Operand dstate, int vblocks, double *partials) {
     extern __shared__ __align__(16) float smem[];
     float *sq = smem, *sk = sq + FC * FLD, *sv = sk + FC * FLD, *sd = sv + FC * 36, *sp = sd + FC * 36, *sz = sp + FC * 36,
           *sm = sz + KM_DECAY_MAX_DIM * 36;
     const int vb = blockIdx.x % vblocks;
-    const int64_t rest = blockIdx.x / vblocks, h = rest % a.heads, seq = rest / a.heads;
+    const unsigned rest = blockIdx.x / (unsigned)vblocks;
+    const int64_t h = rest % a.heads, slot = rest / a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
-    Segment s = {};
-    int64_t begin, length;
-    sequence_rows(a, seq, begin, length);
-    s.seq = (int)seq, s.begin = (int)begin, s.length = (int)length;
+    const Segment s = find_segment(a, slot);
+    if (!s.used || (STATE_ONLY && s.last)) {
+        if (!STATE_ONLY && threadIdx.x == 0) partials[(h * a.slots + slot) * vblocks + vb] = 0.0;
+        return;
+    }
     const int tid = threadIdx.x, tx = tid & 7, ty = tid >> 3;  // columns 4 tx .. + 3, rows ty + 32 i
     const int cols = min(GV, a.dv - vb * GV), dk4 = (a.dk + 3) & ~3;
     const float g2 = log2_decay(a.log_decay[h]);
     Operand v = a.v, d = dout;
     v.data += vb * GV * v.col * (int64_t)sizeof(T);
     d.data += vb * GV * d.col * (int64_t)sizeof(T);
+    const int64_t state = (int64_t)a.dk * a.dv;
+    float *own = a.states + (slot * a.heads + h) * 2 * state + vb * GV;  // Z, then M (where sequences are cut)
     float z[4][4], m[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int r = ty + 32 * i, c = 4 * tx + j;
-            float x = 0.0f;
-            if (a.state_in.data != nullptr && r < a.dk && c < cols)
-                x = exp2f(g2) * a.state_in.at<float>(seq, hg, hi)[r * a.state_in.row + (vb * GV + c) * a.state_in.col];
-            z[i][j] = m[i][j] = x;
+            z[i][j] = m[i][j] = 0.0f;
+            if (STATE_ONLY || r >= a.dk || c >= cols) continue;
+            if (s.first > 0)
+                z[i][j] = own[r * a.dv + c], m[i][j] = own[state + r * a.dv + c];
+            else if (a.state_in.data != nullptr)
+                z[i][j] = m[i][j] = exp2f(g2) * a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + (vb * GV + c) * a.state_in.col];
         }
     double total = 0.0;
-    for (int first = 0; first < s.length; first += FC) {
-        const int tokens = min(FC, s.length - first);
+    for (int first = s.first; first < s.first + s.count; first += FC) {
+        const int tokens = min(FC, s.first + s.count - first);
         const int e = first + tokens == s.length ? tokens - 1 : tokens;
         __syncthreads();
-        load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
+        if (!STATE_ONLY) load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
         load_chunk<T>(sk, a, s, a.k, hg, hi, first, tokens, a.dk, FLD, 128);
         load_chunk<T>(sv, a, s, v, hg, hi, first, tokens, cols, 36, GV);
-        load_chunk<T>(sd, a, s, d, hg, hi, first, tokens, cols, 36, GV);
+        if (!STATE_ONLY) load_chunk<T>(sd, a, s, d, hg, hi, first, tokens, cols, 36, GV);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             *reinterpret_cast<float4 *>(sz + (ty + 32 * i) * 36 + 4 * tx) = make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
@@ -304,7 +311,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
         }
         __syncthreads();
         float sum = 0.0f;
-        {  // inside the chunk: entries (t, u) with t = ty, u = tx + 8 i
+        if (!STATE_ONLY) {  // inside the chunk: entries (t, u) with t = ty, u = tx + 8 i
             float p[4] = {}, r[4] = {};
             for (int c = 0; c < dk4; c += 4) {
                 const float4 x = *reinterpret_cast<const float4 *>(sq + ty * FLD + c);
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
                 if (ty > u) sum = fmaf((float)(ty - u) * exp2f(g2 * (float)(ty - u)) * p[i], r[i], sum);
             }
         }
-        {  // from the states: row t = ty, columns 4 tx ..
+        if (!STATE_ONLY) {  // from the states: row t = ty, columns 4 tx ..
             float x[4] = {}, y[4] = {};
             for (int c = 0; c < a.dk; c++) {
                 const float qv = sq[ty * FLD + c];
@@ -365,7 +372,17 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
             }
         }
     }
-    if (dstate.data != nullptr && s.length > 0) {
+    if (STATE_ONLY) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = ty + 32 * i, c = 4 * tx + j;
+                if (r < a.dk && c < cols) own[r * a.dv + c] = z[i][j], own[state + r * a.dv + c] = m[i][j];
+            }
+        return;
+    }
+    if (dstate.data != nullptr && s.last && s.length > 0) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -373,7 +390,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
                 const int r = ty + 32 * i, c = 4 * tx + j;
                 // (m holds e^{g e} (e Z + M) + ..: the derivative of the last state, whose Z is e^g S_0 with M = Z)
                 if (r < a.dk && c < cols)
-                    total += (double)m[i][j] * (double)dstate.at<float>(seq, hg, hi)[r * dstate.row + (vb * GV + c) * dstate.col];
+                    total += (double)m[i][j] * (double)dstate.at<float>(s.seq, hg, hi)[r * dstate.row + (vb * GV + c) * dstate.col];
             }
     }
     __shared__ double warp_sum[8];
@@ -383,7 +400,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
     __syncthreads();
     if (tid == 0) {
         for (int w = 1; w < 8; w++) total += warp_sum[w];
-        partials[(h * a.sequences + seq) * vblocks + vb] = total;
+        partials[(h * a.slots + slot) * vblocks + vb] = total;
     }
 }
 
@@ -670,16 +687,34 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
 
 namespace km {
 
-// Partial sums, and values of states, of the gradient of the decays.  The kernel on the FMA pipe does not cut sequences:
-// its columns of v are independent, four CTAs to a head.
+// Partial sums, and values of states, of the gradient of the decays.  (On the FMA pipe four CTAs share a head's columns.)
 static size_t grad_sums(const km_decay_problem &p) {
-    const size_t heads = (size_t)(p.groups * p.group);
-    return heads * (p.path == 2 ? (size_t)plan_of(p).slots : (size_t)p.sequences * (size_t)ceil_div(p.dv, GV));
+    return (size_t)(p.groups * p.group) * (size_t)plan_of(p).slots * (size_t)(p.path == 2 ? 1 : ceil_div(p.dv, GV));
 }
 static size_t grad_states(const km_decay_problem &p) {
-    if (p.path != 2) return 0;
     const DecayPlan plan = plan_of(p);
     return plan.split ? (size_t)plan.slots * (size_t)(p.groups * p.group * p.dk * p.dv) * 2 : 0;
+}
+
+template <typename T, bool STATE_ONLY>
+static int launch_grad_fma(const DecayArgs &a, const Operand &d, const Operand &ds, double *partials, cudaStream_t s) {
+    auto kernel = decay_gradient_kernel<T, STATE_ONLY>;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM);
+    if (err != cudaSuccess) return cuda_fail(err, "decay_gradient_kernel");
+    const int vblocks = (int)ceil_div(a.dv, GV);
+    kernel<<<(unsigned)(a.slots * a.heads * vblocks), 256, GRAD_SMEM, s>>>(a, d, ds, vblocks, partials);
+    KM_CHECK_LAUNCH("decay_gradient_kernel launch");
+    return KM_OK;
+}
+
+static int launch_grad(const km_decay_problem &p, const DecayArgs &a, const Operand &d, const Operand &ds, double *partials, bool state_only,
+                       cudaStream_t s) {
+    if (p.path == 2) return launch_decay_grad_tc(p, a, d, ds, partials, state_only, s);
+    if (p.dtype == KM_TYPE_F32)
+        return state_only ? launch_grad_fma<float, true>(a, d, ds, partials, s) : launch_grad_fma<float, false>(a, d, ds, partials, s);
+    if (p.dtype == KM_TYPE_BF16)
+        return state_only ? launch_grad_fma<__nv_bfloat16, true>(a, d, ds, partials, s) : launch_grad_fma<__nv_bfloat16, false>(a, d, ds, partials, s);
+    return state_only ? launch_grad_fma<__half, true>(a, d, ds, partials, s) : launch_grad_fma<__half, false>(a, d, ds, partials, s);
 }
 
 }  // namespace km
@@ -708,34 +743,24 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.scale_in = 1.0f, a.scale_out = p.scale;
     const Operand d = make_operand(dout), ds = make_operand(dstate);
-    const bool tc = p.path == 2;
     a.wait_polls = current_wait_polls();
-    a.gave_up = tc ? gave_up_word() : nullptr;
+    a.gave_up = p.path == 2 ? gave_up_word() : nullptr;
     const DecayPlan plan = plan_of(p);
-    const int vblocks = (int)ceil_div(p.dv, GV);
     const int64_t sums = (int64_t)grad_sums(p) / a.heads, ctas = sums * a.heads;
     KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_gradient: more than 2^31 work items");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     double *partials = static_cast<double *>(workspace);
-    if (ctas > 0 && tc) {
-        a.segment = (unsigned)plan.segment;
-        a.slots = plan.slots;
-        a.states = reinterpret_cast<float *>(partials + ctas);
+    a.segment = (unsigned)plan.segment;
+    a.slots = plan.slots;
+    a.states = reinterpret_cast<float *>(partials + ctas);
+    if (ctas > 0) {
         if (plan.split) {
-            rc = launch_decay_grad_tc(p, a, d, ds, partials, true, s);
-            if (rc == KM_OK) rc = launch_scan<true>(a, s);
+            rc = launch_grad(p, a, d, ds, partials, true, s);
+            if (rc == KM_OK && p.sequences > 0) rc = launch_scan<true>(a, s);
             if (rc != KM_OK) return rc;
         }
-        rc = launch_decay_grad_tc(p, a, d, ds, partials, false, s);
+        rc = launch_grad(p, a, d, ds, partials, false, s);
         if (rc != KM_OK) return rc;
-    } else if (ctas > 0) {
-        auto kernel = p.dtype == KM_TYPE_F32    ? decay_gradient_kernel<float>
-                      : p.dtype == KM_TYPE_BF16 ? decay_gradient_kernel<__nv_bfloat16>
-                                                : decay_gradient_kernel<__half>;
-        cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM);
-        if (err != cudaSuccess) return cuda_fail(err, "decay_gradient_kernel");
-        kernel<<<(unsigned)ctas, 256, GRAD_SMEM, s>>>(a, d, ds, vblocks, partials);
-        KM_CHECK_LAUNCH("decay_gradient_kernel launch");
     }
     decay_gradient_finish_kernel<<<a.heads, 256, 0, s>>>(sums, partials, grad);
     KM_CHECK_LAUNCH("decay_gradient_finish_kernel launch");

@@ -13,18 +13,20 @@
 
 namespace km {
 
-constexpr int NORM_TENSORS = 1024;      // to a launch: 24 KB of parameters
+// Tensors to a launch: 21 KB of parameters, or, where 64 do, 1.3 KB (a launch copies them: 5 us of host time for the long table).
+constexpr int NORM_TENSORS = 1024, NORM_FEW = 64;
 constexpr int64_t NORM_CHUNK = 65536;   // bytes
 constexpr int NORM_CTAS = 148 * 4;
 constexpr int NORM_THREADS = 512;
 
+template <int N>
 struct NormTable {
     int count;
     int64_t chunks;
-    void *data[NORM_TENSORS];
-    int64_t elements[NORM_TENSORS];
-    uint32_t first[NORM_TENSORS];  // number of the tensor's first chunk
-    uint8_t type[NORM_TENSORS];
+    void *data[N];
+    int64_t elements[N];
+    uint32_t first[N];  // number of the tensor's first chunk
+    uint8_t type[N];
 };
 
 struct NormChunk {
@@ -33,7 +35,8 @@ struct NormChunk {
     int type;
 };
 
-__device__ __forceinline__ NormChunk norm_chunk(const NormTable &t, int64_t chunk) {
+template <int N>
+__device__ __forceinline__ NormChunk norm_chunk(const NormTable<N> &t, int64_t chunk) {
     int lo = 0, hi = t.count - 1;  // the last tensor whose first chunk is not behind
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -129,7 +132,8 @@ __device__ __forceinline__ double block_sum(double v, double *scratch) {
     return v;
 }
 
-__global__ void __launch_bounds__(NORM_THREADS) norm_squares_kernel(const __grid_constant__ NormTable t, double *partials) {
+template <int N>
+__global__ void __launch_bounds__(NORM_THREADS) norm_squares_kernel(const __grid_constant__ NormTable<N> t, double *partials) {
     __shared__ double scratch[NORM_THREADS / 32];
     double sum = 0.0;
     for (int64_t chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
@@ -183,7 +187,8 @@ __device__ __forceinline__ void scale_chunk(const NormChunk &c, float f) {
 
 // Every CTA adds the partial sums by itself (a few KB from L2), in the same order.  Chunks are gone through from the last:
 // what the first pass read last may still be in L2.
-__global__ void __launch_bounds__(NORM_THREADS) norm_finish_kernel(const __grid_constant__ NormTable t, const double *partials, int count,
+template <int N>
+__global__ void __launch_bounds__(NORM_THREADS) norm_finish_kernel(const __grid_constant__ NormTable<N> t, const double *partials, int count,
                                                                   int scale, double max_norm, double eps, float *norm) {
     __shared__ double scratch[NORM_THREADS / 32];
     grid_wait();
@@ -206,6 +211,46 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_finish_kernel(const __grid_
     }
 }
 
+template <int N>
+static int norm_launches(int64_t count, void *const *tensors, const int64_t *elements, const int32_t *types, int32_t scale_in_place, double max_norm,
+                         double eps, float *norm, double *partials, cudaStream_t s) {
+    static thread_local NormTable<N> table;  // (which a launch copies)
+    int used = 0;
+    const auto fill = [&](int64_t first) -> int {
+        table.count = 0, table.chunks = 0;
+        for (int64_t i = first; i < std::min(count, first + N); i++) {
+            if (elements[i] == 0) continue;
+            const int j = table.count++;
+            table.data[j] = tensors[i], table.elements[j] = elements[i], table.type[j] = (uint8_t)types[i];
+            table.first[j] = (uint32_t)table.chunks;
+            table.chunks += ceil_div(elements[i], NORM_CHUNK / (types[i] == KM_TYPE_F32 ? 4 : 2));
+            KM_REQUIRE(table.chunks < (1LL << 32), KM_ERR_UNSUPPORTED, "km_global_norm: more than 2^48 bytes");
+        }
+        return KM_OK;
+    };
+    const int64_t launches = std::max<int64_t>(1, ceil_div(count, N));
+    for (int64_t l = 0; l < launches; l++) {
+        const int rc = fill(l * N);
+        if (rc != KM_OK) return rc;
+        const int ctas = (int)std::min<int64_t>(table.chunks, NORM_CTAS);
+        if (ctas == 0) continue;
+        norm_squares_kernel<N><<<ctas, NORM_THREADS, 0, s>>>(table, partials + used);
+        KM_CHECK_LAUNCH("norm_squares_kernel launch");
+        used += ctas;
+    }
+    for (int64_t l = 0; l < (scale_in_place ? launches : 1); l++) {
+        if (launches > 1) {
+            const int rc = fill(l * N);
+            if (rc != KM_OK) return rc;
+        }
+        const int ctas = scale_in_place ? (int)std::max<int64_t>(1, std::min<int64_t>(table.chunks, NORM_CTAS)) : 1;
+        const int rc = launch_chained("norm_finish_kernel launch", norm_finish_kernel<N>, dim3((unsigned)ctas), NORM_THREADS, 0, s, table,
+                                      (const double *)partials, used, (int)scale_in_place, max_norm, eps, l == 0 ? norm : (float *)nullptr);
+        if (rc != KM_OK) return rc;
+    }
+    return KM_OK;
+}
+
 }  // namespace km
 
 extern "C" size_t km_global_norm_workspace_bytes(int64_t count) {
@@ -226,41 +271,6 @@ extern "C" int km_global_norm(int64_t count, void *const *tensors, const int64_t
         KM_REQUIRE(reinterpret_cast<uintptr_t>(tensors[i]) % (types[i] == KM_TYPE_F32 ? 4 : 2) == 0 && elements[i] < (1LL << 40),
                    KM_ERR_INVALID_ARGUMENT, "km_global_norm: bad tensor %lld", (long long)i);
     }
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    double *partials = static_cast<double *>(workspace);
-    static thread_local NormTable table;  // (24 KB that a launch copies)
-    int used = 0;
-    const auto fill = [&](int64_t first) -> int {
-        table.count = 0, table.chunks = 0;
-        for (int64_t i = first; i < std::min(count, first + NORM_TENSORS); i++) {
-            if (elements[i] == 0) continue;
-            const int j = table.count++;
-            table.data[j] = tensors[i], table.elements[j] = elements[i], table.type[j] = (uint8_t)types[i];
-            table.first[j] = (uint32_t)table.chunks;
-            table.chunks += ceil_div(elements[i], NORM_CHUNK / (types[i] == KM_TYPE_F32 ? 4 : 2));
-            KM_REQUIRE(table.chunks < (1LL << 32), KM_ERR_UNSUPPORTED, "km_global_norm: more than 2^48 bytes");
-        }
-        return KM_OK;
-    };
-    const int64_t launches = std::max<int64_t>(1, ceil_div(count, NORM_TENSORS));
-    for (int64_t l = 0; l < launches; l++) {
-        const int rc = fill(l * NORM_TENSORS);
-        if (rc != KM_OK) return rc;
-        const int ctas = (int)std::min<int64_t>(table.chunks, NORM_CTAS);
-        if (ctas == 0) continue;
-        norm_squares_kernel<<<ctas, NORM_THREADS, 0, s>>>(table, partials + used);
-        KM_CHECK_LAUNCH("norm_squares_kernel launch");
-        used += ctas;
-    }
-    for (int64_t l = 0; l < (scale_in_place ? launches : 1); l++) {
-        if (launches > 1) {
-            const int rc = fill(l * NORM_TENSORS);
-            if (rc != KM_OK) return rc;
-        }
-        const int ctas = scale_in_place ? (int)std::max<int64_t>(1, std::min<int64_t>(table.chunks, NORM_CTAS)) : 1;
-        const int rc = launch_chained("norm_finish_kernel launch", norm_finish_kernel, dim3((unsigned)ctas), NORM_THREADS, 0, s, table,
-                                      (const double *)partials, used, (int)scale_in_place, max_norm, eps, l == 0 ? norm : (float *)nullptr);
-        if (rc != KM_OK) return rc;
-    }
-    return KM_OK;
+    const auto run = count <= NORM_FEW ? km::norm_launches<NORM_FEW> : km::norm_launches<NORM_TENSORS>;
+    return run(count, tensors, elements, types, scale_in_place, max_norm, eps, norm, static_cast<double *>(workspace), static_cast<cudaStream_t>(stream));
 }

@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
 template <typename T>
 static int launch_rotary(RotaryArgs &a, int64_t batch, bool wide, bool interleaved, cudaStream_t s) {
     constexpr int VEC = 16 / sizeof(T);
-    // tokens of a CTA: four CTAs' worth of tokens per SM where there are that many, else fewer to a CTA; the table of
-    // angles stays within 32 KB
+    // Four tokens to a CTA where that still gives four CTAs per SM, else fewer: with 16 the last, partly filled wave of CTAs
+    // costs too much (335 MB: 72 us; 8: 64, 4: 62.5, 2: 66).
     const int64_t rows = batch * a.tokens;
-    a.tile = (int)std::max<int64_t>(1, std::min<int64_t>({16, rows / (4 * 148), 4096 / std::max(a.pairs, 1)}));
+    a.tile = (int)std::max<int64_t>(1, std::min<int64_t>(4, rows / (4 * 148)));
     const int64_t ctas = batch * ceil_div(a.tokens, a.tile);
     KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_rotary: more than 2^31 work items");
     auto kernel = wide ? (interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>)
