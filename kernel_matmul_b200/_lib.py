@@ -34,7 +34,8 @@ class KmDecayProblem(ctypes.Structure):
     _fields_ = [
         ("dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("reverse", ctypes.c_int32), ("path", ctypes.c_int32),
         ("sequences", ctypes.c_int64), ("tokens", ctypes.c_int64), ("groups", ctypes.c_int64), ("group", ctypes.c_int64),
-        ("dk", ctypes.c_int64), ("dv", ctypes.c_int64), ("packed", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("dk", ctypes.c_int64), ("dv", ctypes.c_int64), ("packed", ctypes.c_int32), ("states", ctypes.c_int32),
+        ("scale", ctypes.c_float),
     ]
 
 

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
             float x = 0.0f;
             if (!STATE_ONLY && r < a.dk && c < a.dv) {
                 if (!first_segment)
-                    x = a.states[((slot * a.heads + h) * a.dk + r) * a.dv + c];
+                    x = a.states[((int64_t)s.start * a.heads + h) * a.dk * a.dv + r * a.state_row + c * a.state_col];
                 else if (a.state_in.data != nullptr)
                     x = a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + c * a.state_in.col];
             }
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
                 const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
                 if (r >= a.dk || c >= a.dv) continue;
                 if (STATE_ONLY)
-                    a.states[((slot * a.heads + h) * a.dk + r) * a.dv + c] = z[i][j];
+                    a.states[(((int64_t)s.adds * a.heads + h) * a.dk + r) * a.dv + c] = z[i][j];
                 else
                     a.state_out.at<float>(s.seq, hg, hi)[r * a.state_out.row + c * a.state_out.col] = z[i][j];
             }
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// States at the start of each segment, in place: states[slot] held the segment's own contribution.  A thread takes four
+// States at the start of each segment but the first, in place of what the segments before them add.  A thread takes four
 // values of the state through the segments of a sequence, four segments loaded ahead: all is read and written once.
 //
 // TANGENT: of Z and, behind it, M = dZ/dg:  M <- e^{g n} (n Z + M) + own, n = tokens of a segment.
@@ -208,8 +208,9 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
     const int slot0 = segments_before(a, seq);
     int64_t begin, length;
     sequence_rows(a, seq, begin, length);
-    const int n = min(segments_of(a, length), (int)a.slots - slot0);
-    if (n <= 1) return;
+    const int place = slot0 - (int)seq;
+    const int n = (int)min((int64_t)segments_of(a, length) - 1, a.state_slots - place);
+    if (n <= 0) return;
     const float g2 = log2_decay(a.log_decay[h]);
     const float carry = exp2f(g2 * (float)a.segment), enter = a.reverse ? 1.0f : exp2f(g2);
     const int values = a.dk * a.dv, first = blockIdx.y * 1024 + threadIdx.x;
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
                           ? enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col]
                           : 0.0f;
     }
-    float *p = a.states + ((int64_t)slot0 * a.heads + h) * N * values + first;
+    float *p = a.states + ((int64_t)place * a.heads + h) * N * values + first;
     const int64_t step = (int64_t)a.heads * N * values;
     const float tokens = (float)a.segment;
     for (int j = 0; j < n; j += 4) {
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
         for (int u = 0; u < 4; u++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const bool there = j + u + 1 < n && first + 256 * c < values;
+                const bool there = j + u < n && first + 256 * c < values;
                 own[u][c] = there ? p[(j + u) * step + 256 * c] : 0.0f;
                 own_m[u][c] = TANGENT && there ? p[(j + u) * step + values + 256 * c] : 0.0f;
             }
@@ -239,12 +240,12 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
         for (int u = 0; u < 4; u++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                if (j + u > 0 && j + u < n && first + 256 * c < values) {
+                if (TANGENT) m[c] = fmaf(carry, fmaf(tokens, z[c], m[c]), own_m[u][c]);
+                z[c] = fmaf(carry, z[c], own[u][c]);
+                if (j + u < n && first + 256 * c < values) {
                     p[(j + u) * step + 256 * c] = z[c];
                     if (TANGENT) p[(j + u) * step + values + 256 * c] = m[c];
                 }
-                if (TANGENT) m[c] = fmaf(carry, fmaf(tokens, z[c], m[c]), own_m[u][c]);
-                z[c] = fmaf(carry, z[c], own[u][c]);
             }
     }
 }
@@ -281,7 +282,9 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
     v.data += vb * GV * v.col * (int64_t)sizeof(T);
     d.data += vb * GV * d.col * (int64_t)sizeof(T);
     const int64_t state = (int64_t)a.dk * a.dv;
-    float *own = a.states + (slot * a.heads + h) * 2 * state + vb * GV;  // Z, then M (where sequences are cut)
+    // Z, then M, where sequences are cut
+    float *own = a.states + ((int64_t)s.adds * a.heads + h) * 2 * state + vb * GV;
+    const float *start = a.states + ((int64_t)s.start * a.heads + h) * 2 * state + vb * GV;
     float z[4][4], m[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
             z[i][j] = m[i][j] = 0.0f;
             if (STATE_ONLY || r >= a.dk || c >= cols) continue;
             if (s.first > 0)
-                z[i][j] = own[r * a.dv + c], m[i][j] = own[state + r * a.dv + c];
+                z[i][j] = start[r * a.dv + c], m[i][j] = start[state + r * a.dv + c];
             else if (a.state_in.data != nullptr)
                 z[i][j] = m[i][j] = exp2f(g2) * a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + (vb * GV + c) * a.state_in.col];
         }
@@ -548,7 +551,7 @@ static int sm_count() {
 
 struct DecayPlan {
     bool tc, split;
-    int64_t segment, slots;
+    int64_t segment, slots, states;  // states: places for those between segments, at most
 };
 
 static DecayPlan plan_of(const km_decay_problem &p) {
@@ -573,6 +576,7 @@ static DecayPlan plan_of(const km_decay_problem &p) {
     r.segment = per * chunk;
     r.split = per < chunks;
     r.slots = p.packed ? p.tokens / r.segment + p.sequences : p.sequences * ceil_div(std::max<int64_t>(p.tokens, 1), r.segment);
+    r.states = r.split ? std::max<int64_t>(r.slots - p.sequences, 1) : 0;
     return r;
 }
 
@@ -582,6 +586,7 @@ static int check_problem(const char *name, const km_decay_problem *p) {
                KM_ERR_INVALID_ARGUMENT, "%s: bad element type", name);
     KM_REQUIRE(p->path == 1 || (p->path == 2 && p->dtype != KM_TYPE_F32), KM_ERR_UNSUPPORTED,
                "%s: path must be 1 (FMA pipe) or, for 16-bit types, 2 (tensor cores)", name);
+    KM_REQUIRE(p->states >= 0 && p->states <= 2, KM_ERR_INVALID_ARGUMENT, "%s: states must be 0, 1 or 2", name);
     KM_REQUIRE(p->sequences >= 0 && p->tokens >= 0 && p->groups >= 0 && p->group >= 1, KM_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
     KM_REQUIRE(p->dk >= 1 && p->dk <= KM_DECAY_MAX_DIM && p->dv >= 1 && p->dv <= KM_DECAY_MAX_DIM, KM_ERR_UNSUPPORTED,
                "%s: head sizes must be 1 to %d", name, KM_DECAY_MAX_DIM);
@@ -645,7 +650,7 @@ extern "C" size_t km_decay_attention_workspace_bytes(const km_decay_problem *pro
     const km_decay_problem p = resolved(*problem);
     if (check_problem("km_decay_attention_workspace_bytes", &p) != KM_OK) return 0;
     const DecayPlan plan = plan_of(p);
-    return plan.split ? (size_t)plan.slots * (size_t)(p.groups * p.group * p.dk * p.dv) * 4 : 0;
+    return (size_t)plan.states * (size_t)(p.groups * p.group * p.dk * p.dv) * 4;
 }
 
 extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view *q, const km_view *k, const km_view *v, const km_view *out,
@@ -669,6 +674,8 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     a.segment = (unsigned)plan.segment;
     a.slots = plan.slots;
     a.states = static_cast<float *>(workspace);
+    a.state_slots = plan.states;
+    a.state_row = p.states == 2 ? 1 : (int)p.dv, a.state_col = p.states == 2 ? (int)p.dk : 1;
     a.scale_in = p.reverse ? p.scale : 1.0f;
     a.scale_out = p.reverse ? 1.0f : p.scale;
     a.reverse = p.reverse != 0;
@@ -676,7 +683,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     a.gave_up = plan.tc ? gave_up_word() : nullptr;
     KM_REQUIRE(a.slots * a.heads < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_attention: more than 2^31 work items");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (plan.split) {
+    if (plan.split && p.states == 0) {
         rc = launch_main(p, a, plan.tc, true, s);
         if (rc != KM_OK) return rc;
         rc = launch_scan<false>(a, s);
@@ -692,8 +699,7 @@ static size_t grad_sums(const km_decay_problem &p) {
     return (size_t)(p.groups * p.group) * (size_t)plan_of(p).slots * (size_t)(p.path == 2 ? 1 : ceil_div(p.dv, GV));
 }
 static size_t grad_states(const km_decay_problem &p) {
-    const DecayPlan plan = plan_of(p);
-    return plan.split ? (size_t)plan.slots * (size_t)(p.groups * p.group * p.dk * p.dv) * 2 : 0;
+    return (size_t)plan_of(p).states * (size_t)(p.groups * p.group * p.dk * p.dv) * 2;
 }
 
 template <typename T, bool STATE_ONLY>
@@ -752,6 +758,7 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
     double *partials = static_cast<double *>(workspace);
     a.segment = (unsigned)plan.segment;
     a.slots = plan.slots;
+    a.state_slots = plan.states;
     a.states = reinterpret_cast<float *>(partials + ctas);
     if (ctas > 0) {
         if (plan.split) {

@@ -39,7 +39,11 @@ struct DecayArgs {
     int dk, dv;
     unsigned segment;       // tokens of a segment (a multiple of the chunk; the sums of tokens and a segment fit 32 bits)
     int64_t slots;          // segments of all sequences, at most (less than 2^31, as all counts of this file)
-    float *states;          // one (dk, dv) per (slot, head): the state a segment starts with (gradient of the decays: two, Z and M)
+    // What a segment adds to its sequence's state, then (decay_scan_kernel) the state the next one starts with: state_slots x heads
+    // of (dk, dv) (gradient of the decays: two, Z and M); values (r, c) at r state_row + c state_col.
+    float *states;
+    int64_t state_slots;
+    int state_row, state_col;
     float scale_in, scale_out;  // on k v^T, and on the result
     int reverse;
     int *gave_up;
@@ -73,6 +77,7 @@ __device__ __forceinline__ float log2_decay(float g) {
 struct Segment {
     int seq, begin, length;  // its sequence: number, first row, rows (of all three there are less than 2^31)
     int first, count;        // its tokens inside the sequence (in the order in which they are gone through)
+    int adds, start;         // places in `states` of what it adds (not of a last segment) and of its start (not of a first one)
     int spare, spares;       // rows of no sequence are shared by `spares` CTAs per head, of which this is number `spare`; -1: none
     bool used, last;
 };
@@ -156,6 +161,9 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot
     r.begin = (int)begin, r.length = (int)length;
     r.first = index * (int)a.segment;
     r.last = index == segments_of(a, length) - 1;
+    // (a sequence of n segments has n - 1 states; bounded, should `starts` decrease and sequences overlap)
+    r.adds = (int)min(slot - r.seq, a.state_slots - 1);
+    r.start = (int)min(slot - r.seq - 1, a.state_slots - 1);
     r.count = min(r.length - r.first, (int)a.segment);
     // the very last slot is in use: its CTA sees to the rows of no sequence
     if (a.starts != nullptr && slot == a.slots - 1) r.spare = 0, r.spares = 1;

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
         const bool state_row = row < VB * 64;
         const int64_t state = (int64_t)a.dk * a.dv;
-        float *own = a.states + (slot * a.heads + h) * 2 * state;  // Z, then M (where sequences are cut)
+        float *own = a.states + ((int64_t)s.adds * a.heads + h) * 2 * state;  // Z, then M (where sequences are cut)
         f32x2 z[NZ / 2], m[NZ / 2];
         {
             const float *from = nullptr, *from_m = nullptr;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             float enter = 1.0f;
             if (!STATE_ONLY && row < a.dv) {
                 if (s.first > 0) {
-                    from = own + row, from_m = from + state, step = a.dv;
+                    from = a.states + ((int64_t)s.start * a.heads + h) * 2 * state + row, from_m = from + state, step = a.dv;
                 } else if (a.state_in.data != nullptr) {
                     from = from_m = a.state_in.at<const float>(s.seq, hg, hi) + row * a.state_in.col;
                     step = a.state_in.row, enter = exp2f(g2);

@@ -369,8 +369,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
         int64_t step = 0;
         if (!STATE_ONLY && row < a.dv) {
             if (!first_segment) {
-                from = a.states + (slot * a.heads + h) * (int64_t)a.dk * a.dv + row;
-                step = a.dv;
+                from = a.states + ((int64_t)s.start * a.heads + h) * a.dk * a.dv + row * a.state_col;
+                step = a.state_row;
             } else if (a.state_in.data != nullptr) {
                 from = a.state_in.at<const float>(s.seq, hg, hi) + row * a.state_in.col;
                 step = a.state_in.row;
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
             mbar_arrive(&ctl.q_empty[b]);
         }
         if (row < a.dv && (STATE_ONLY || (s.last && a.state_out.data != nullptr))) {
-            float *to = STATE_ONLY ? a.states + (slot * a.heads + h) * (int64_t)a.dk * a.dv + row
+            float *to = STATE_ONLY ? a.states + ((int64_t)s.adds * a.heads + h) * a.dk * a.dv + row
                                    : a.state_out.at<float>(s.seq, hg, hi) + row * a.state_out.col;
             const int64_t row_step = STATE_ONLY ? a.dv : a.state_out.row;
 #pragma unroll

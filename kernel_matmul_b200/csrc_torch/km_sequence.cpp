@@ -202,29 +202,32 @@ struct DecayCall {
     }
     const int32_t *starts_ptr() const { return starts.defined() ? starts.const_data_ptr<int32_t>() : nullptr; }
 
-    void run(bool reverse, bool transposed, const Tensor &a, const Tensor &b, const Tensor &c, const Tensor &out, const Tensor &state_in,
-             const Tensor &state_out) const {
-        const km_decay_problem p = problem(reverse, transposed, out.scalar_type() == at::kFloat);
+    // `states`: the workspace of a call over the same states with dk and dv swapped (undefined: none).  Returns this call's own.
+    Tensor run(bool reverse, bool transposed, const Tensor &a, const Tensor &b, const Tensor &c, const Tensor &out, const Tensor &state_in,
+               const Tensor &state_out, const Tensor &states = Tensor()) const {
+        km_decay_problem p = problem(reverse, transposed, out.scalar_type() == at::kFloat);
         if (sequences == 0) {  // (no launch will write the rows of no sequence)
             out.zero_();
-            return;
+            return Tensor();
         }
         const km_view va = tokens_view(a), vb = tokens_view(b), vc = tokens_view(c), vo = tokens_view(out),
                       vi = state_view(state_in, transposed), vs = state_view(state_out, transposed);
         const size_t bytes = km_decay_attention_workspace_bytes(&p);
-        const Tensor ws = bytes ? workspace(q, bytes) : Tensor();
+        p.states = bytes && states.defined() ? 2 : 0;
+        const Tensor ws = !bytes ? Tensor() : p.states ? states : workspace(q, bytes);
         raise_on(km_decay_attention(&p, &va, &vb, &vc, &vo, log_decay.const_data_ptr<float>(), starts_ptr(), &vi, &vs,
                                     bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+        return ws;
     }
     Tensor state_like() const { return at::empty({sequences, heads, dk, dv}, q.options().dtype(at::kFloat).requires_grad(false)); }
     Tensor result_like() const { return at::empty({q.size(0), tokens, heads, dv}, q.options().requires_grad(false)); }
     // per-head results of `dim` values summed over the heads of a group
     Tensor summed(bool transposed, const Tensor &a, const Tensor &b, const Tensor &c, int64_t dim, const Tensor &state_in,
-                  const Tensor &state_out) const {
+                  const Tensor &state_out, Tensor &states) const {
         const auto opt = q.options().requires_grad(false);
         const int64_t group = heads / groups;
         Tensor out = at::empty({q.size(0), tokens, heads, dim}, group > 1 ? opt.dtype(at::kFloat) : opt);
-        run(true, transposed, a, b, c, out, state_in, state_out);
+        states = run(true, transposed, a, b, c, out, state_in, state_out, states);
         if (group == 1) return out;
         Tensor sums = at::empty({q.size(0), tokens, groups, dim}, opt);
         raise_on(km_group_sums(type, q.size(0) * tokens, groups, group, dim, out.const_data_ptr<float>(), sums.data_ptr(), stream_of(q)));
@@ -232,11 +235,12 @@ struct DecayCall {
     }
 };
 
-static variable_list decay_forward(const DecayCall &c, bool return_state) {
+static variable_list decay_forward(const DecayCall &c, bool return_state, Tensor *states = nullptr) {
     const c10::cuda::CUDAGuard guard(c.q.device());
     poll_gave_up(c.q.device().index());
     Tensor out = c.result_like(), state = return_state ? c.state_like() : Tensor();
-    c.run(false, false, c.q, c.k, c.v, out, c.initial, state);
+    const Tensor ws = c.run(false, false, c.q, c.k, c.v, out, c.initial, state);
+    if (states != nullptr) *states = ws;
     return return_state ? variable_list{out, state} : variable_list{out};
 }
 
@@ -245,11 +249,13 @@ struct DecayFunction : torch::autograd::Function<DecayFunction> {
                                  const Maybe &initial, const Maybe &starts, const DecayCall &call, bool return_state) {
         DecayCall c = call;  // (the inputs as the function sees them)
         c.q = q, c.k = k, c.v = v, c.log_decay = log_decay, c.initial = initial.value_or(Tensor()), c.starts = starts.value_or(Tensor());
-        ctx->save_for_backward({q, k, v, log_decay, c.initial, c.starts});
+        Tensor states;  // between segments, for the gradient of q
+        variable_list out = decay_forward(c, return_state, &states);
+        ctx->save_for_backward({q, k, v, log_decay, c.initial, c.starts, states});
         ctx->saved_data["sizes"] = std::vector<int64_t>{c.sequences, c.tokens, c.heads, c.groups, c.dk, c.dv, c.path, c.type};
         ctx->saved_data["scale"] = c.scale;
         ctx->set_materialize_grads(false);
-        return decay_forward(c, return_state);
+        return out;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "decay_attention has no second derivative (create_graph)");
@@ -265,14 +271,15 @@ struct DecayFunction : torch::autograd::Function<DecayFunction> {
         if (!go.defined()) go = at::zeros({1}, c.q.options().requires_grad(false)).expand({c.q.size(0), c.tokens, c.heads, c.dv});
         if (ctx->needs_input_grad(0)) {
             out[0] = at::empty(c.q.sizes(), c.q.options().requires_grad(false));
-            c.run(false, true, go, c.v, c.k, out[0], c.initial, Tensor());
+            c.run(false, true, go, c.v, c.k, out[0], c.initial, Tensor(), s[6]);
         }
-        if (ctx->needs_input_grad(1)) out[1] = c.summed(true, c.v, go, c.q, c.dk, ds, Tensor());
         const bool initial = c.initial.defined() && ctx->needs_input_grad(4);
+        Tensor back;  // the states of the way back, which the gradients of v and k share
         if (ctx->needs_input_grad(2) || initial) {
             if (initial) out[4] = c.state_like();
-            out[2] = c.summed(false, c.k, c.q, go, c.dv, ds, out[4]);
+            out[2] = c.summed(false, c.k, c.q, go, c.dv, ds, out[4], back);
         }
+        if (ctx->needs_input_grad(1)) out[1] = c.summed(true, c.v, go, c.q, c.dk, ds, Tensor(), back);
         if (ctx->needs_input_grad(3)) {
             const km_decay_problem p = c.problem(false, false, false);
             out[3] = at::empty({c.heads}, c.log_decay.options().requires_grad(false));

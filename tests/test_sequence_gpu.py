@@ -52,6 +52,8 @@ CASES = [
     dict(lengths=[900, 3, 0, 1500], tail=0, heads=3, groups=3, dk=40, dv=128, decay="mixed"),
     dict(lengths=[0, 0], tail=9, heads=2, groups=2, dk=16, dv=16),
     dict(lengths=[17] * 70, tail=300, heads=2, groups=2, dk=32, dv=32),
+    dict(lengths=[3, 5000, 0, 1, 2600], tail=1, heads=2, groups=1, dk=64, dv=128),
+    dict(batch=2, tokens=3000, heads=2, groups=2, dk=128, dv=40),
 ]
 
 
@@ -569,3 +571,18 @@ def test_refusals():
                lambda: ops.decay_attention(q, k, v, g, path="nodes")):
         with pytest.raises(ValueError):
             f_()
+
+
+def test_sequence_starts_that_decrease_stay_inside():
+    """Sequences that overlap are not supported: their results are undefined, but nothing is read or written out of range, and
+    other tensors keep their values."""
+    t = 5000
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v = (randn(t, 2, 64, dtype=dtype).requires_grad_() for _ in range(3))
+        g = decays(2).requires_grad_()
+        guard = [torch.full((1 << 20,), 7.0, device=DEV) for _ in range(4)]
+        for starts in ([0, t, 0, t, 0, t], [t, 0], [0, t, -3, t + 50, 10, 5, t]):
+            o, s = ops.decay_attention(q, k, v, g, sequence_starts=torch.tensor(starts, dtype=torch.int32, device=DEV), return_state=True)
+            torch.autograd.grad(o.sum() + s.sum(), [q, k, v, g])
+        ops.check()
+        assert all((x == 7.0).all() for x in guard)
