@@ -586,3 +586,43 @@ def test_sequence_starts_that_decrease_stay_inside():
             torch.autograd.grad(o.sum() + s.sum(), [q, k, v, g])
         ops.check()
         assert all((x == 7.0).all() for x in guard)
+
+
+@pytest.fixture
+def short_waits():
+    """A function that makes every hand-off wait of the tensor-core kernels give up at its first test."""
+    from kernel_matmul_b200._lib import lib
+
+    try:
+        yield lambda: lib.km_selftest_set_wait_polls(0)
+    finally:
+        assert lib.km_selftest_set_wait_polls(-1) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,dim", [(100, 64), (1000, 128), (3000, 40)])
+def test_attention_that_gives_up_reports_and_poisons_its_results(dtype, tokens, dim, short_waits):
+    from kernel_matmul_b200._lib import lib
+
+    q, k, v = (randn(2, tokens, 2, dim, dtype=dtype).requires_grad_() for _ in range(3))
+    g = decays(2).requires_grad_()
+    inputs = [q, k, v, g]
+    o, s = ops.decay_attention(q, k, v, g, return_state=True)
+    cotangents = [torch.randn_like(o), torch.randn_like(s)]
+    want = torch.autograd.grad([o, s], inputs, cotangents, retain_graph=True)
+    torch.cuda.synchronize()
+    assert short_waits() == 0
+    bad, bad_state = (x.detach() for x in ops.decay_attention(q, k, v, g, return_state=True))
+    torch.cuda.synchronize()  # the launches end by themselves
+    assert torch.isnan(bad).all() and torch.isnan(bad_state).all()
+    with pytest.raises(ops.KernelGaveUpError, match="decay_attention"):
+        ops.check()
+    grads = torch.autograd.grad([o, s], inputs, cotangents, retain_graph=True)
+    torch.cuda.synchronize()
+    assert all(torch.isnan(x).all() for x in grads)
+    with pytest.raises(ops.KernelGaveUpError):
+        ops.check()
+    assert lib.km_selftest_set_wait_polls(-1) == 0
+    again = torch.autograd.grad([o, s], inputs, cotangents)
+    ops.check()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
