@@ -679,6 +679,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     a.scale_in = p.reverse ? p.scale : 1.0f;
     a.scale_out = p.reverse ? 1.0f : p.scale;
     a.reverse = p.reverse != 0;
+    a.parts = p.dtype == KM_TYPE_BF16 ? 3 : 2;
     a.wait_polls = current_wait_polls();
     a.gave_up = plan.tc ? gave_up_word() : nullptr;
     KM_REQUIRE(a.slots * a.heads < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_attention: more than 2^31 work items");

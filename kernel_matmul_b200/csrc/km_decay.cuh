@@ -46,6 +46,7 @@ struct DecayArgs {
     int state_row, state_col;
     float scale_in, scale_out;  // on k v^T, and on the result
     int reverse;
+    int parts;                  // 16-bit parts of the decayed keys on the tensor cores
     int *gave_up;
     unsigned wait_polls;
 };

@@ -1,15 +1,15 @@
 // Gradient of the log decays on the tensor cores (km_decay.cu, decay_gradient_kernel, has the formula and why it takes a second
 // state): 16-bit operands, chunks of 128 tokens, one CTA per (sequence, head).
 //
-// The gradient is an fp32 sum, so nothing of it may be rounded to 16 bits but the decayed operands, which go in two parts
-// (2^-17 in bf16).  Per chunk, with d = t - s, e the exponent of the chunk's end and all accumulators fp32:
+// The gradient is an fp32 sum, so nothing of it may be rounded to 16 bits but the decayed operands, which go in parts: two in fp16
+// (2^-22), three in bf16 (2^-25).  Per chunk, with d = t - s, e the exponent of the chunk's end and all accumulators fp32:
 //   S = Q K^T, G = dO V^T:  sum over s < t of d e^{g d} S G, entry by entry in registers
 //   U  = V^T K~, U' = V^T K':       K~ = e^{g (e - s)} K,  K' = (e - s) e^{g (e - s)} K
 //   X  = dO^T Q~, X' = dO^T Q':     Q~ = e^{g t} Q,        Q' = t e^{g t} Q
 //   sum += <X', Z> + <X, M>,  M <- e^{g e} (e Z + M) + U',  Z <- e^{g e} Z + U   with Z and M in registers
 // (the products of the states with q and then dO are sums over the tokens first, so that neither state is an operand).
-// Ten products of 128^3 with their parts, 5100 cycles of the tensor pipe per chunk of a head with dk = dv = 128: the phases
-// follow one another, eight warps of arithmetic and one that loads and multiplies; there is no room for a second stage.
+// Fourteen products of 128^3 with the three parts, 7200 cycles of the tensor pipe per chunk of a head with dk = dv = 128, and between
+// them the parts have to be written into the only three tiles that Q, K, V and dO leave: the phases follow one another.
 #include "km_decay_tc.cuh"
 
 namespace km {
@@ -26,7 +26,7 @@ struct GradMaps {
 };
 
 struct GradControl {
-    uint64_t full, sg_full, k_ready, u_full, q_ready, x_full, read, drain;
+    uint64_t full, sg_full, ready, done, read, drain;
     uint32_t tmem;
     int dead;
     float inner[16];  // 2^(g2 (15 - j))
@@ -40,29 +40,26 @@ struct GradSmem {
     static_assert(BYTES <= 232448, "shared memory of an SM");
 };
 
-// The decayed operand in two parts and, weighted with `more` besides, in two further ones; 16 bytes of each.
-template <typename T>
-__device__ __forceinline__ void decayed_parts(uint4 x, float w, float more, uint4 (&out)[4]) {
+// 16 bytes of an operand times w in PARTS parts, each to its own tile.
+template <typename T, int PARTS>
+__device__ __forceinline__ void write_parts(uint4 x, float w, unsigned char *tile, int bytes) {
     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-    uint32_t r[4][4];
+    uint32_t r[PARTS][4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const float2 v = unpack<T>(in[j]);
         f32x2 y = mul2(pack2(v.x, v.y), splat2(w));
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < PARTS; i++) {
             float y0, y1;
             unpack2(y, y0, y1);
-            r[2 * i][j] = pack<T>(y0, y1);
-            const float2 h = unpack<T>(r[2 * i][j]);
-            float l0, l1;
-            unpack2(sub2(y, pack2(h.x, h.y)), l0, l1);
-            r[2 * i + 1][j] = pack<T>(l0, l1);
-            y = mul2(y, splat2(more));
+            r[i][j] = pack<T>(y0, y1);
+            const float2 h = unpack<T>(r[i][j]);
+            y = sub2(y, pack2(h.x, h.y));
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) out[i] = make_uint4(r[i][0], r[i][1], r[i][2], r[i][3]);
+    for (int i = 0; i < PARTS; i++) *reinterpret_cast<uint4 *>(tile + i * bytes) = make_uint4(r[i][0], r[i][1], r[i][2], r[i][3]);
 }
 
 }  // namespace
@@ -73,6 +70,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                                                                         const __grid_constant__ Operand dstate,
                                                                         const __grid_constant__ GradMaps maps, double *partials) {
     using L = GradSmem<KB, VB>;
+    constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
     constexpr int NZ = KB * 16;  // of the states' rows: this thread's columns
     constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
     extern __shared__ unsigned char raw[];
@@ -88,8 +86,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = (s.count + TC - 1) / TC;
     const float g2 = log2_decay(a.log_decay[h]);
     if (tid == 0) {
-        mbar_init(&ctl.full, 33), mbar_init(&ctl.sg_full, 1), mbar_init(&ctl.u_full, 1), mbar_init(&ctl.x_full, 1), mbar_init(&ctl.drain, 1);
-        mbar_init(&ctl.k_ready, ARITH), mbar_init(&ctl.q_ready, ARITH), mbar_init(&ctl.read, ARITH);
+        mbar_init(&ctl.full, 33), mbar_init(&ctl.sg_full, 1), mbar_init(&ctl.done, 1), mbar_init(&ctl.drain, 1);
+        mbar_init(&ctl.ready, ARITH), mbar_init(&ctl.read, ARITH);
         ctl.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -109,13 +107,14 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
         unsigned bytes = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) bytes += maps.use[i] && !(STATE_ONLY && (i == 0 || i == 3)) ? (i < 2 ? KB : VB) * BLOCK_BYTES : 0;
-        // sum over the tokens of A^T B: A (values on the lanes) and B's parts as they lie in memory
-        const auto outer = [&](uint32_t col, uint32_t a_at, uint32_t high, uint32_t low) {
-            const uint64_t at = tile_desc(base + a_at, VB == 2 ? NEXT : 0), ht = tile_desc(base + high, NEXT), lt = tile_desc(base + low, NEXT);
-#pragma unroll 2
-            for (int ks = 0; ks < TC / 16; ks++) {
-                mma_ss(tmem + col, at + ks * 128, ht + ks * 128, idesc_u, ks > 0);
-                mma_ss(tmem + col, at + ks * 128, lt + ks * 128, idesc_u, 1u);
+        // sum over the tokens of A^T B: A (values on the lanes) as it lies in memory, B in parts
+        const auto outer = [&](uint32_t col, uint32_t a_at) {
+            const uint64_t at = tile_desc(base + a_at, VB == 2 ? NEXT : 0);
+#pragma unroll 1
+            for (int i = PARTS - 1; i >= 0; i--) {  // (small parts first: the tensor cores cut a sum's last bits off at every step)
+                const uint64_t bt = tile_desc(base + L::SPARE + i * KB * BLOCK_BYTES, NEXT);
+#pragma unroll
+                for (int ks = 0; ks < TC / 16; ks++) mma_ss(tmem + col, at + ks * 128, bt + ks * 128, idesc_u, i < PARTS - 1 || ks > 0);
             }
         };
         const auto inner = [&](uint32_t col, uint32_t x, uint32_t y, int blocks) {
@@ -125,7 +124,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                 mma_ss(tmem + col, xd + at, yd + at, idesc_sg, ks > 0);
             }
         };
-        const uint32_t spare[3] = {(uint32_t)L::SPARE, (uint32_t)(L::SPARE + KB * BLOCK_BYTES), (uint32_t)(L::SPARE + 2 * KB * BLOCK_BYTES)};
+        constexpr int PHASES = STATE_ONLY ? 2 : 4;  // U, U', X, X'
+        unsigned phase = 0;
         bool ok = true;
         int filled = 0;
         for (int it = 0; it < chunks && ok; it++) {
@@ -158,29 +158,17 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                 mma_commit(&ctl.sg_full);
             }
             __syncwarp();
-            ok = mbar_wait_warp(&ctl.k_ready, it & 1, a.wait_polls);
-            if (!ok) break;
-            tc_fence_after();
-            if (lane == 0) {
-                outer(COL_U, L::V, L::K, spare[0]);
-                outer(COL_U1, L::V, spare[1], spare[2]);
-                mma_commit(&ctl.u_full);
+            for (int i = 0; i < PHASES && ok; i++, phase++) {
+                ok = mbar_wait_warp(&ctl.ready, phase & 1, a.wait_polls);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    outer(i == 0 ? COL_U : i == 1 ? COL_U1 : i == 2 ? COL_G : COL_S, i < 2 ? L::V : L::D);
+                    mma_commit(&ctl.done);
+                }
+                __syncwarp();
+                ok = mbar_wait_warp(&ctl.done, phase & 1, a.wait_polls);
             }
-            __syncwarp();
-            if (STATE_ONLY) {
-                ok = mbar_wait_warp(&ctl.u_full, it & 1, a.wait_polls);
-                continue;
-            }
-            ok = mbar_wait_warp(&ctl.q_ready, it & 1, a.wait_polls);
-            if (!ok) break;
-            tc_fence_after();
-            if (lane == 0) {
-                outer(COL_G, L::D, L::Q, spare[0]);
-                outer(COL_S, L::D, spare[1], spare[2]);
-                mma_commit(&ctl.x_full);
-            }
-            __syncwarp();
-            ok = mbar_wait_warp(&ctl.x_full, it & 1, a.wait_polls);
         }
         if (!ok) ctl.dead = 1;
         // no copy and no product may be in flight when the CTA ends
@@ -216,6 +204,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             }
         }
         double total = 0.0;
+        unsigned phase = 0;
         bool ok = true;
         for (int it = 0; it < chunks; it++) {
             const int tokens = min(TC, s.count - it * TC);
@@ -228,18 +217,21 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             if (tokens < TC)  // rows behind the chunk may be another sequence's: not even 0 * inf may come in
                 for (int p = tid; p < (STATE_ONLY ? 1 : 2) * VB * TC * 8; p += ARITH)
                     if (((p >> 3) & (TC - 1)) >= tokens) *reinterpret_cast<uint4 *>(smem + L::V + p * 16) = make_uint4(0, 0, 0, 0);
+            // an operand times `weight` of its token, in parts
+            const auto parts = [&](int tile, auto weight) {
 #pragma unroll 2
-            for (int p = tid; p < KB * TC * 8; p += ARITH) {
-                const int t = (p >> 3) & (TC - 1);
-                uint4 x = *reinterpret_cast<const uint4 *>(smem + L::K + p * 16), out[4];
-                if (t >= tokens) x = make_uint4(0, 0, 0, 0);
-                decayed_parts<T>(x, exp2f(g2 * (float)max(last - t, 0)), (float)max(e - t, 0) * PART, out);
-                *reinterpret_cast<uint4 *>(smem + L::K + p * 16) = out[0];
-#pragma unroll
-                for (int i = 0; i < 3; i++) *reinterpret_cast<uint4 *>(smem + L::SPARE + i * KB * BLOCK_BYTES + p * 16) = out[i + 1];
-            }
-            fence_async_smem();
-            mbar_arrive(&ctl.k_ready);
+                for (int p = tid; p < KB * TC * 8; p += ARITH) {
+                    const int t = (p >> 3) & (TC - 1);
+                    uint4 x = *reinterpret_cast<const uint4 *>(smem + tile + p * 16);
+                    if (t >= tokens) x = make_uint4(0, 0, 0, 0);
+                    write_parts<T, PARTS>(x, weight(t), smem + L::SPARE + p * 16, KB * BLOCK_BYTES);
+                }
+                fence_async_smem();
+                mbar_arrive(&ctl.ready);
+            };
+            const auto before_last = [&](int t) { return exp2f(g2 * (float)max(last - t, 0)); };
+            const auto behind_first = [&](int t) { return exp2f(g2 * (float)t); };
+            parts(L::K, before_last);
             // (under the products U)
             f32x2 sum = splat2(0.0f);
             if (!STATE_ONLY) {
@@ -250,7 +242,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                     tmem_ld16_nowait(lanes + COL_G + c0, y);
                     const int d = row - c0;
                     const bool diagonal = c0 + 31 >= r0 + 16;  // (blocks of 16 columns that reach the diagonal of the warp's rows)
-                    const f32x2 outer = splat2(ex2_approx(g2 * (float)max(d - 15, 0)));
+                    const f32x2 outer = splat2(exp2f(g2 * (float)max(d - 15, 0)));
                     tmem_ld_wait16(x);
                     tmem_ld_wait16(y);
 #pragma unroll
@@ -275,22 +267,17 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                 }
             }
             tc_fence_before();  // (S and G have been read before X goes over them)
-            ok = mbar_wait_warp(&ctl.u_full, it & 1, a.wait_polls);
+            ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
+            if (!ok) break;
+            parts(L::K, [&](int t) { return before_last(t) * ((float)max(e - t, 0) * PART); });
+            ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
             if (!ok) break;
             if (!STATE_ONLY) {
-#pragma unroll 2
-                for (int p = tid; p < KB * TC * 8; p += ARITH) {
-                    const int t = (p >> 3) & (TC - 1);
-                    uint4 x = *reinterpret_cast<const uint4 *>(smem + L::Q + p * 16), out[4];
-                    if (t >= tokens) x = make_uint4(0, 0, 0, 0);
-                    decayed_parts<T>(x, exp2f(g2 * (float)t), (float)t * PART, out);
-                    *reinterpret_cast<uint4 *>(smem + L::Q + p * 16) = out[0];
-#pragma unroll
-                    for (int i = 0; i < 3; i++) *reinterpret_cast<uint4 *>(smem + L::SPARE + i * KB * BLOCK_BYTES + p * 16) = out[i + 1];
-                }
-                fence_async_smem();
-                mbar_arrive(&ctl.q_ready);
-                ok = mbar_wait_warp(&ctl.x_full, it & 1, a.wait_polls);
+                parts(L::Q, behind_first);
+                ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
+                if (!ok) break;
+                parts(L::Q, [&](int t) { return behind_first(t) * ((float)t * PART); });
+                ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
                 if (!ok) break;
             }
             tc_fence_after();

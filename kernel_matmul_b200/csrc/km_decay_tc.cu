@@ -3,19 +3,27 @@
 // and fp32 accumulators in tensor memory (128 lanes):
 //   S  = Q K^T            operands as they are in memory; lanes are tokens t
 //   QZ = Q Z              Z: the state in 16 bits (below), dv x dk in shared memory
-//   PV = P V              P = S with decays and mask, in 16 bits, from tensor memory
-//   U  = V^T K~           K~ = K with decays e^{g (e - s)}, in two 16-bit parts; lanes are columns of v
+//   U  = V^T K~           K~ = K with decays to the chunk's last token, in parts (below); lanes are columns of v
+//   PV = P V              P = S with decays and mask, in two 16-bit parts, from tensor memory
 //   out = PV + e^{g t} QZ,  Z <- e^{g e} Z + U     in fp32
 // The tiles of Q, K and V have ONE layout, rows of 64 values (128 bytes, 128-byte swizzle), which the matrix unit takes either
 // along the values (Q, K in S) or along the tokens (V in PV, V and K~ in U): nothing is transposed.
 //
-// Roundings to 16 bits: P and the state's copy in QZ, each once per term, half a step of the operands' type: as large as the
-// rounding of the result.  Z itself and U stay in fp32; K~ = hi + lo (2^-17 relative in bf16), since its sum is the state, an fp32
-// result.  fp16 has too few exponents for P and Z: both are scaled by powers of two per row, taken back in fp32.
+// Roundings to 16 bits.  The state's copy in QZ is rounded once, half a step of the operands' type (its low part has no room in
+// shared memory): the only one, besides the result's own, and as large as that.  P goes in two parts (one part made results of
+// short sequences 1.4 - 1.6 times as wrong as their rounding).  Z itself and U stay in fp32 and are fp32 results: K~ goes in two
+// parts in fp16 (2^-22) and three in bf16 (2^-25).  The tensor cores cut the last bits of a sum off at every step of 16 tokens,
+// so small parts are added up first: final states are within 1.5e-7 (2-norm, as an fp32 evaluation is) instead of 5e-7, and
+// 2.4e-6 with two parts of bf16.  fp16 has too few exponents for P and Z: both are scaled by powers of two per row, taken back in
+// fp32.
 //
-// Bound by memory: a chunk of a head with dk = dv = 128 moves 128 KB and takes five products of 128^3 (1300 cycles of the tensor
-// pipe), while its share of HBM takes 5600 cycles.  So everything is about keeping loads in flight: two stages of Q, K, V (96 KB
-// each), filled through TMA; K~ goes over K and Q once S and QZ have read them, P over S.
+// What bounds it: a chunk of a head with dk = dv = 128 moves 128 KB, 5600 cycles of its SM's share of HBM, but 670 KB through
+// shared memory (products of 128^3 with both operands there take 64 KB each), 5200 cycles at 128 bytes each, and its phases depend
+// on one another: S, then P and K~, then the products with V, then the next state and QZ.  They take 8000 cycles, or 6400 with one part
+// of P and two of K~ (148 heads x 4096 tokens: 158 and 129 us, 3.9 and 4.8 TB/s of operands).  Three kinds of warps work at once on
+// neighbouring phases; two stages of Q, K, V are filled through TMA; K~ goes over K, Q and Z once the products have read them, P
+// over S.  What did not help: S of the next chunk before U, results drained from registers while U runs, K~ made before S is there
+// (all within 3 %: shared memory is what they wait for).
 #include "km_decay_tc.cuh"
 
 namespace km {
@@ -25,15 +33,17 @@ namespace {
 constexpr int GROUP = 256;    // threads of a group: two per lane of tensor memory
 // warps 0 - 7: results and state; 8 - 15: operands; 16: matrix products; 17, 18: loads; 19: none
 constexpr int MMA_WARP = 16, THREADS = 640;
-// Registers: 640 threads are launched with 96 each, 61 440 in all, which the groups divide: 256 x 128 + 256 x 72 + 128 x 80.
+// Registers: 640 threads are launched with 96 each, 61 440 in all, which the groups divide: 256 x 144 + 256 x 64 + 128 x 64.
 constexpr int RESULT_REGS = 144, OPERAND_REGS = 64, OTHER_REGS = 64;
 static_assert(256 * RESULT_REGS + 256 * OPERAND_REGS + 128 * OTHER_REGS <= THREADS * 96, "registers at launch");
+
 template <int KB, int VB>
 struct Smem {
     // (the Q tile is also where the results leave through: 8 warps' 4 KB)
     static constexpr int Q = 0, K = 2 * BLOCK_BYTES, V = K + KB * BLOCK_BYTES, STAGE = V + VB * BLOCK_BYTES;
-    static constexpr int Z = 2 * STAGE;                       // KB blocks of (64 VB rows of 64 values)
-    static constexpr int REST = Z + KB * VB * 64 * 128;
+    // the state: KB blocks of (64 VB rows of 64 values); between its product with q and its next value a third part of K~
+    static constexpr int Z = 2 * STAGE;
+    static constexpr int REST = Z + KB * BLOCK_BYTES;
     static constexpr int BYTES = 1024 + REST;
 };
 
@@ -228,15 +238,24 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 const uint64_t vd = tile_desc(base + b * L::STAGE + L::V, BLOCK_BYTES);
                 const uint64_t vt = tile_desc(base + b * L::STAGE + L::V, VB == 2 ? BLOCK_BYTES : 0);  // (VB = 1: lanes 64 .. 127 repeat 0 .. 63)
                 const uint64_t kt = tile_desc(base + b * L::STAGE + L::K, BLOCK_BYTES), lt = tile_desc(base + b * L::STAGE + L::Q, BLOCK_BYTES);
+                // (the tensor cores cut a sum's last bits off at every step: small parts first, so that most steps have little to lose)
+                bool begun = false;
+                if (!HALF && a.parts == 3) {
+                    const uint64_t zt = tile_desc(base + L::Z, BLOCK_BYTES);
 #pragma unroll
-                for (int ks = 0; ks < TC / 16; ks++) {
-                    mma_ss(tmem + COL_U, vt + ks * 128, kt + ks * 128, idesc_u, ks > 0);
-                    mma_ss(tmem + COL_U, vt + ks * 128, lt + ks * 128, idesc_u, 1u);
+                    for (int ks = 0; ks < TC / 16; ks++) mma_ss(tmem + COL_U, vt + ks * 128, zt + ks * 128, idesc_u, ks > 0);
+                    begun = true;
                 }
+#pragma unroll
+                for (int ks = 0; ks < TC / 16; ks++) mma_ss(tmem + COL_U, vt + ks * 128, lt + ks * 128, idesc_u, begun || ks > 0);
+#pragma unroll
+                for (int ks = 0; ks < TC / 16; ks++) mma_ss(tmem + COL_U, vt + ks * 128, kt + ks * 128, idesc_u, 1u);
                 if (!STATE_ONLY) {
 #pragma unroll
-                    for (int ks = 0; ks < TC / 16; ks++)
-                        mma_f16_ts(tmem + COL_PV, tmem + COL_S + ks * 16, vd + ks * 128, idesc_pv, ks > 0);
+                    for (int i = 8; i >= 0; i -= 8)  // P's low part, then its high part
+#pragma unroll
+                        for (int ks = 0; ks < TC / 16; ks++)
+                            mma_f16_ts(tmem + COL_PV, tmem + COL_S + ks * 16 + i, vd + ks * 128, idesc_pv, i == 0 || ks > 0);
                 }
                 mma_commit(&ctl.o_full);
                 mma_commit(&ctl.empty[b]);
@@ -292,10 +311,10 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
 #pragma unroll 1
                 for (int c0 = half * 16; c0 < TC; c0 += 32) {
                     const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
-                    uint32_t w[8];
+                    uint32_t w[16];  // eight words of high parts, eight of low ones
                     if (side > 0) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++) w[j] = 0;
+                        for (int j = 0; j < 16; j++) w[j] = 0;
                     } else {
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
@@ -308,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                                 const float2 inner = *reinterpret_cast<const float2 *>(&ctl.inner[2 * j]);
                                 float u, v;
                                 unpack2(mul2(mul2(pack2(inner.x, inner.y), outer), pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))), u, v);
-                                w[j] = pack<T>(u, v);
+                                two_parts<T>(u, v, w[j], w[j + 8]);
                             }
                         } else {  // entry by entry
                             const f32x2 g22 = splat2(a.reverse ? -g2 : g2), d2 = splat2((float)d), up2 = splat2(up);
@@ -318,16 +337,18 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                                 const f32x2 x = ex2_approx2(mul2(g22, sub2(d2, pack2((float)(2 * j), (float)(2 * j + 1)))));
                                 float u, v;
                                 unpack2(mul2(HALF ? mul2(x, up2) : x, pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))), u, v);
-                                w[j] = pack<T>((a.reverse ? 2 * j >= d : 2 * j <= d) ? u : 0.0f, (a.reverse ? 2 * j + 1 >= d : 2 * j + 1 <= d) ? v : 0.0f);
+                                two_parts<T>((a.reverse ? 2 * j >= d : 2 * j <= d) ? u : 0.0f, (a.reverse ? 2 * j + 1 >= d : 2 * j + 1 <= d) ? v : 0.0f,
+                                             w[j], w[j + 8]);
                             }
                         }
                     }
-                    tmem_st8(lanes + COL_S + c0, w);  // (over the first 8 of the 16 columns that have been read)
+                    tmem_st16(lanes + COL_S + c0, w);  // (over the 16 columns that have been read)
                 }
                 tmem_st_wait();
                 tc_fence_before();
             }
-            // K~ over K, its low part over Q, which QZ has read by now
+            // K~ over K, its low part over Q and, if there is one, its lowest over Z, which QZ has read by now
+            const bool three = !HALF && a.parts == 3;
             if (!STATE_ONLY) {
                 ok = mbar_wait_warp(&ctl.qz_full, it & 1, a.wait_polls);
                 if (!ok) break;
@@ -341,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 if (m >= tokens) x = make_uint4(0, 0, 0, 0);
                 const f32x2 w = splat2(exp2f(g2 * (float)max(a.reverse ? m : tokens - 1 - m, 0)));  // decay to the chunk's last token
                 const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-                uint32_t high[4], low[4];
+                uint32_t high[4], low[4], lowest[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float2 v = unpack<T>(in[j]);
@@ -349,10 +370,17 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                     float y0, y1;
                     unpack2(y, y0, y1);
                     high[j] = pack<T>(y0, y1);
-                    const float2 r = unpack<T>(high[j]);
-                    unpack2(sub2(y, pack2(r.x, r.y)), y0, y1);
+                    float2 r = unpack<T>(high[j]);
+                    const f32x2 rest = sub2(y, pack2(r.x, r.y));
+                    unpack2(rest, y0, y1);
                     low[j] = pack<T>(y0, y1);
+                    if (!HALF) {
+                        r = unpack<T>(low[j]);
+                        unpack2(sub2(rest, pack2(r.x, r.y)), y0, y1);
+                        lowest[j] = pack<T>(y0, y1);
+                    }
                 }
+                if (three) *reinterpret_cast<uint4 *>(smem + L::Z + mine * 16 + i * (GROUP * 16)) = make_uint4(lowest[0], lowest[1], lowest[2], lowest[3]);
                 *reinterpret_cast<uint4 *>(kt + i * (GROUP * 16)) = make_uint4(high[0], high[1], high[2], high[3]);
                 *reinterpret_cast<uint4 *>(qt + i * (GROUP * 16)) = make_uint4(low[0], low[1], low[2], low[3]);
             }

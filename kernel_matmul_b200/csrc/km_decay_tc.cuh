@@ -56,13 +56,6 @@ __device__ __forceinline__ void tmem_ld_wait8x2(uint32_t (&p)[8], uint32_t (&q)[
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 :
-                 : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
-
 // two values as one word, the first in the low half, rounded to nearest
 template <typename T>
 __device__ __forceinline__ uint32_t pack(float a, float b);
@@ -85,6 +78,14 @@ __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
     return __half22float2(reinterpret_cast<const __half2 &>(w));
+}
+
+// Two values in two parts: high (rounded to nearest) and what that leaves.
+template <typename T>
+__device__ __forceinline__ void two_parts(float a, float b, uint32_t &high, uint32_t &low) {
+    high = pack<T>(a, b);
+    const float2 h = unpack<T>(high);
+    low = pack<T>(a - h.x, b - h.y);
 }
 
 // Whether every row starts on a boundary of 16 bytes.
