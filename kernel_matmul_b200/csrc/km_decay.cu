@@ -14,16 +14,21 @@ constexpr int FC = 32;          // tokens of a chunk
 constexpr int FLD = 132;        // floats of a row of q, k, v in shared memory
 constexpr int FMA_SMEM = (3 * FC * FLD + FC * 36 + KM_DECAY_MAX_DIM * KM_DECAY_MAX_DIM) * 4;
 
-template <typename T>
+// Rows [first, first + tokens) of an operand into shared memory, zeros behind them and behind `dim`.  A thread's values are all under
+// way before the first is stored (one after the other they took a chunk 15 us).
+template <typename T, int LD, int WIDTH>
 __device__ __forceinline__ void load_chunk(float *dst, const DecayArgs &a, const Segment &s, const Operand &o, int64_t hg, int64_t hi,
-                                           int first, int tokens, int dim, int ld, int width) {
+                                           int first, int tokens, int dim) {
+    constexpr int STEP = 256 / WIDTH, N = FC / STEP;
     const T *src = o.at<T>(a.starts == nullptr ? s.seq : 0, hg, hi);
-    for (int i = threadIdx.x; i < FC * width; i += blockDim.x) {
-        const int t = i / width, c = i - t * width;
-        float x = 0.0f;
-        if (t < tokens && c < dim) x = as_float(src[token_row(a, s, first + t) * o.row + c * o.col]);
-        dst[t * ld + c] = x;
-    }
+    const int c = threadIdx.x % WIDTH, t0 = threadIdx.x / WIDTH;
+    const T *p = src + token_row(a, s, first + t0) * o.row + c * o.col;
+    const int64_t step = (a.reverse ? -STEP : STEP) * o.row;
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = t0 + i * STEP < tokens && c < dim ? as_float(p[i * step]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) dst[(t0 + i * STEP) * LD + c] = x[i];
 }
 
 template <typename T, typename O, bool STATE_ONLY>
@@ -78,9 +83,9 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
         const bool final = first + tokens == s.length;
         const int e = final && !a.reverse ? tokens - 1 : tokens;
         __syncthreads();
-        if (!STATE_ONLY) load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
-        load_chunk<T>(sk, a, s, a.k, hg, hi, first, tokens, a.dk, FLD, 128);
-        load_chunk<T>(sv, a, s, a.v, hg, hi, first, tokens, a.dv, FLD, 128);
+        if (!STATE_ONLY) load_chunk<T, FLD, 128>(sq, a, s, a.q, hg, hi, first, tokens, a.dk);
+        load_chunk<T, FLD, 128>(sk, a, s, a.k, hg, hi, first, tokens, a.dk);
+        load_chunk<T, FLD, 128>(sv, a, s, a.v, hg, hi, first, tokens, a.dv);
         if (!STATE_ONLY) {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -303,10 +308,10 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
         const int tokens = min(FC, s.first + s.count - first);
         const int e = first + tokens == s.length ? tokens - 1 : tokens;
         __syncthreads();
-        if (!STATE_ONLY) load_chunk<T>(sq, a, s, a.q, hg, hi, first, tokens, a.dk, FLD, 128);
-        load_chunk<T>(sk, a, s, a.k, hg, hi, first, tokens, a.dk, FLD, 128);
-        load_chunk<T>(sv, a, s, v, hg, hi, first, tokens, cols, 36, GV);
-        if (!STATE_ONLY) load_chunk<T>(sd, a, s, d, hg, hi, first, tokens, cols, 36, GV);
+        if (!STATE_ONLY) load_chunk<T, FLD, 128>(sq, a, s, a.q, hg, hi, first, tokens, a.dk);
+        load_chunk<T, FLD, 128>(sk, a, s, a.k, hg, hi, first, tokens, a.dk);
+        load_chunk<T, 36, GV>(sv, a, s, v, hg, hi, first, tokens, cols);
+        if (!STATE_ONLY) load_chunk<T, 36, GV>(sd, a, s, d, hg, hi, first, tokens, cols);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             *reinterpret_cast<float4 *>(sz + (ty + 32 * i) * 36 + 4 * tx) = make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
@@ -563,8 +568,9 @@ static DecayPlan plan_of(const km_decay_problem &p) {
     // time again and some chunks' worth of launches.
     int64_t per = chunks;
     if (p.packed) {
-        // lengths are known on the device only: segments of which all sequences together give two per SM
-        per = std::min(chunks, std::max<int64_t>(4, ceil_div(chunks * heads, 2 * sms)));
+        // lengths are known on the device only: segments of which all sequences together give two per SM, but of no fewer than
+        // eight chunks, for which two further launches do not pay
+        per = std::min(chunks, std::max<int64_t>(8, ceil_div(chunks * heads, 2 * sms)));
     } else {
         double best = (double)ceil_div(p.sequences * heads, sms) * (double)(chunks + 2);
         for (int64_t n = 2; n <= 64 && n <= chunks; n++) {

@@ -175,6 +175,18 @@ struct DecayCall {
         p.scale = (float)scale;
         return p;
     }
+    // An operand of the tensor-core kernels, which load rows that start on boundaries of 16 bytes by TMA and any others value by
+    // value: those are copied into such rows first, but for sequences of a few tokens (4 heads of 33 and 77: 500 tokens take
+    // 159 us without the copies and 48 with them, 64 tokens 46 and 36; a token's three copies cost 10 us of host time).
+    Tensor ready(const Tensor &t) const {
+        if (type == KM_TYPE_F32 || path == PATH_FMA || t.size(1) < 16) return t;
+        bool aligned = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+        for (int64_t d = 0; d < 3; d++) aligned = aligned && (t.size(d) == 1 || (t.stride(d) % 8 == 0 && (d != 1 || t.stride(d) > 0)));
+        if (aligned) return t;
+        at::NoGradGuard no_grad;
+        const Tensor rows = at::empty({t.size(0), t.size(1), t.size(2), (t.size(3) + 7) / 8 * 8}, t.options().requires_grad(false)).narrow(3, 0, t.size(3));
+        return rows.copy_(t);
+    }
     // (sequence, token, head, value) with all heads, or one for each group
     km_view tokens_view(const Tensor &t) const {
         km_view v{};
@@ -203,8 +215,9 @@ struct DecayCall {
     const int32_t *starts_ptr() const { return starts.defined() ? starts.const_data_ptr<int32_t>() : nullptr; }
 
     // `states`: the workspace of a call over the same states with dk and dv swapped (undefined: none).  Returns this call's own.
-    Tensor run(bool reverse, bool transposed, const Tensor &a, const Tensor &b, const Tensor &c, const Tensor &out, const Tensor &state_in,
+    Tensor run(bool reverse, bool transposed, const Tensor &ta, const Tensor &tb, const Tensor &tc, const Tensor &out, const Tensor &state_in,
                const Tensor &state_out, const Tensor &states = Tensor()) const {
+        const Tensor a = ready(ta), b = ready(tb), c = ready(tc);
         km_decay_problem p = problem(reverse, transposed, out.scalar_type() == at::kFloat);
         if (sequences == 0) {  // (no launch will write the rows of no sequence)
             out.zero_();
@@ -248,10 +261,10 @@ struct DecayFunction : torch::autograd::Function<DecayFunction> {
     static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                                  const Maybe &initial, const Maybe &starts, const DecayCall &call, bool return_state) {
         DecayCall c = call;  // (the inputs as the function sees them)
-        c.q = q, c.k = k, c.v = v, c.log_decay = log_decay, c.initial = initial.value_or(Tensor()), c.starts = starts.value_or(Tensor());
+        c.q = c.ready(q), c.k = c.ready(k), c.v = c.ready(v), c.log_decay = log_decay, c.initial = initial.value_or(Tensor()), c.starts = starts.value_or(Tensor());
         Tensor states;  // between segments, for the gradient of q
         variable_list out = decay_forward(c, return_state, &states);
-        ctx->save_for_backward({q, k, v, log_decay, c.initial, c.starts, states});
+        ctx->save_for_backward({c.q, c.k, c.v, log_decay, c.initial, c.starts, states});
         ctx->saved_data["sizes"] = std::vector<int64_t>{c.sequences, c.tokens, c.heads, c.groups, c.dk, c.dv, c.path, c.type};
         ctx->saved_data["scale"] = c.scale;
         ctx->set_materialize_grads(false);
@@ -269,8 +282,9 @@ struct DecayFunction : torch::autograd::Function<DecayFunction> {
         const c10::cuda::CUDAGuard guard(c.q.device());
         poll_gave_up(c.q.device().index());
         if (!go.defined()) go = at::zeros({1}, c.q.options().requires_grad(false)).expand({c.q.size(0), c.tokens, c.heads, c.dv});
+        go = c.ready(go);
         if (ctx->needs_input_grad(0)) {
-            out[0] = at::empty(c.q.sizes(), c.q.options().requires_grad(false));
+            out[0] = at::empty({c.q.size(0), c.tokens, c.heads, c.dk}, c.q.options().requires_grad(false));
             c.run(false, true, go, c.v, c.k, out[0], c.initial, Tensor(), s[6]);
         }
         const bool initial = c.initial.defined() && ctx->needs_input_grad(4);

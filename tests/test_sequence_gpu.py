@@ -626,3 +626,37 @@ def test_attention_that_gives_up_reports_and_poisons_its_results(dtype, tokens, 
     again = torch.autograd.grad([o, s], inputs, cotangents)
     ops.check()
     assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_training_step_in_a_graph():
+    """Forward pass, gradients and clipping captured and replayed with other values in the same buffers."""
+    q, k, v = (randn(2, 200, 2, 64, dtype=torch.bfloat16).requires_grad_() for _ in range(3))
+    g = decays(2).requires_grad_()
+    frequencies, _ = ops.rotary_frequencies(64)
+    positions = torch.arange(200, device=DEV)
+
+    def step():
+        a, b = ops.rotary(q, k, positions, frequencies)
+        o = ops.decay_attention(a, b, v, g)
+        grads = list(torch.autograd.grad(o.float().square().mean(), [q, k, v, g]))
+        return [o.detach(), *grads, ops.clip_global_norm_(grads, 0.01)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        with torch.no_grad():
+            for t in (q, k, v):
+                t.copy_(randn(*t.shape, dtype=t.dtype))
+        graph.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
