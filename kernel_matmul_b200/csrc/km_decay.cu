@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
         __syncthreads();
         if (!STATE_ONLY) {
             float p[2][2] = {};
+#pragma unroll 2
             for (int c = 0; c < dk4; c += 4) {
                 float4 x[2], y[2];
 #pragma unroll
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
                 }
             __syncthreads();
             float o[2][8] = {};
+#pragma unroll 4
             for (int c = 0; c < a.dk; c++) {
                 const float4 z0 = *reinterpret_cast<const float4 *>(sz + c * 128 + 4 * tx);
                 const float4 z1 = *reinterpret_cast<const float4 *>(sz + c * 128 + 4 * tx + 64);
@@ -141,6 +143,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) o[i][j] *= w;
             }
+#pragma unroll 4
             for (int u = 0; u < tokens; u++) {
                 const float4 v0 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx);
                 const float4 v1 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx + 64);
@@ -172,6 +175,7 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
         for (int i = 0; i < 8; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) z[i][j] *= carry;
+#pragma unroll 4
         for (int u = 0; u < tokens; u++) {
             const float w = exp2f(g2 * (float)(e - u)) * a.scale_in;
             const float4 v0 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx);
@@ -345,6 +349,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
         }
         if (!STATE_ONLY) {  // from the states: row t = ty, columns 4 tx ..
             float x[4] = {}, y[4] = {};
+#pragma unroll 4
             for (int c = 0; c < a.dk; c++) {
                 const float qv = sq[ty * FLD + c];
                 const float4 zz = *reinterpret_cast<const float4 *>(sz + c * 36 + 4 * tx);
@@ -367,6 +372,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
                 m[i][j] = carry * fmaf((float)e, z[i][j], m[i][j]);
                 z[i][j] *= carry;
             }
+#pragma unroll 4
         for (int u = 0; u < tokens; u++) {
             const float w = exp2f(g2 * (float)(e - u)), wm = w * (float)(e - u);
             const float4 vv = *reinterpret_cast<const float4 *>(sv + u * 36 + 4 * tx);
