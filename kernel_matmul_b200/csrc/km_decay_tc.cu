@@ -349,10 +349,11 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
             }
             // K~ over K, its low part over Q and, if there is one, its lowest over Z, which QZ has read by now
             const bool three = !HALF && a.parts == 3;
-            if (!STATE_ONLY) {
+            if (!STATE_ONLY)
                 ok = mbar_wait_warp(&ctl.qz_full, it & 1, a.wait_polls);
-                if (!ok) break;
-            }
+            else if (three && it > 0)  // (nothing but U of the chunk before holds Z's only tile)
+                ok = mbar_wait_warp(&ctl.o_full, (it - 1) & 1, a.wait_polls);
+            if (!ok) break;
             unsigned char *kt = smem + b * L::STAGE + L::K + mine * 16, *qt = smem + b * L::STAGE + L::Q + mine * 16;
 #pragma unroll
             for (int i = 0; i < KB * 4; i++) {

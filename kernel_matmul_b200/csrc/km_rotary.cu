@@ -113,7 +113,7 @@ static int launch_rotary(RotaryArgs &a, int64_t batch, bool wide, bool interleav
     // Four tokens to a CTA where that still gives four CTAs per SM, else fewer: with 16 the last, partly filled wave of CTAs
     // costs too much (335 MB: 72 us; 8: 64, 4: 62.5, 2: 66).
     const int64_t rows = batch * a.tokens;
-    a.tile = (int)std::max<int64_t>(1, std::min<int64_t>(4, rows / (4 * 148)));
+    a.tile = (int)std::max<int64_t>(1, std::min<int64_t>({4, rows / (4 * 148), 4096 / std::max(a.pairs, 1)}));  // (32 KB of angles at most)
     const int64_t ctas = batch * ceil_div(a.tokens, a.tile);
     KM_REQUIRE(ctas < (1LL << 31), KM_ERR_UNSUPPORTED, "km_rotary: more than 2^31 work items");
     auto kernel = wide ? (interleaved ? rotary_kernel<T, VEC, true> : rotary_kernel<T, VEC, false>)

@@ -355,7 +355,7 @@ def test_step_strided_states():
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("tokens,heads,groups,dim,turned", [(1, 1, 1, 2, 2), (33, 4, 2, 64, 64), (700, 3, 1, 80, 40), (65, 2, 2, 7, 6), (129, 8, 8, 128, 96), (9, 2, 1, 16, 0)])
+@pytest.mark.parametrize("tokens,heads,groups,dim,turned", [(1, 1, 1, 2, 2), (33, 4, 2, 64, 64), (700, 3, 1, 80, 40), (65, 2, 2, 7, 6), (129, 8, 8, 128, 96), (9, 2, 1, 16, 0), (1500, 2, 1, 4096, 4096)])
 def test_rotary(dtype, interleaved, tokens, heads, groups, dim, turned):
     q, k = randn(2, tokens, heads, dim, dtype=dtype), randn(2, tokens, groups, dim, dtype=dtype)
     frequencies, scale = ops.rotary_frequencies(turned, scaling="parts", factor=4.0, original_tokens=2048)
@@ -660,3 +660,20 @@ def test_training_step_in_a_graph():
             want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_gives_the_same_bits_again(dtype):
+    """Sums are added up in a fixed order, and no hand-off between warps is left to chance."""
+    cases = [(2, 3000, 4, 2, 128, 128), (1, 9000, 2, 2, 64, 128), (3, 700, 4, 4, 128, 64), (1, 5000, 3, 3, 64, 64)]
+    for b, t, h, groups, dk, dv in cases:
+        q, k, v = randn(b, t, h, dk, dtype=dtype), randn(b, t, groups, dk, dtype=dtype), randn(b, t, groups, dv, dtype=dtype)
+        g, s0 = decays(h), randn(b, h, dk, dv)
+        inputs = [x.requires_grad_() for x in (q, k, v, g, s0)]
+        go, gs = randn(b, t, h, dv, dtype=dtype), randn(b, h, dk, dv)
+        want = None
+        for _ in range(8):
+            o, s = ops.decay_attention(q, k, v, g, initial_state=s0, return_state=True)
+            got = [o.detach(), s.detach(), *torch.autograd.grad([o, s], inputs, [go, gs])]
+            assert want is None or all(torch.equal(a, c) for a, c in zip(got, want))
+            want = got
