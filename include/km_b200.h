@@ -593,8 +593,9 @@ KM_API int km_rotary(int32_t dtype, int64_t batch, int64_t tokens, const int64_t
  * i.e. the product of the matrix e^{g (t - s)} (q_t . k_s), s <= t, which is generated on the fly, with v.
  *
  * `reverse`: the same backwards in time, in the form of a gradient: with W_t = scale k_t v_t^T + e^g W_{t+1},
- * where e^g W_{len} is state_in as it is, out_t = W_t^T q_t, and state_out = e^g W_0.  With (q, k, v, state_in):
- *   dq = forward (dout, v, k, S_0^T),  dk = reverse (v, dout, q, dS^T),  dv and dS_0 = reverse (k, q, dout, dS).
+ * where e^g W_{len} is state_in as it is, out_t = W_t^T q_t, and state_out = e^g W_0.  reverse = 2: forwards, as a part of a
+ * gradient that returns no state.  With (q, k, v, state_in):
+ *   dq = forward, reverse = 2, (dout, v, k, S_0^T),  dk = reverse (v, dout, q, dS^T),  dv and dS_0 = reverse (k, q, dout, dS).
  *
  * Sequences are batches of `tokens` rows, or, with `starts` (sequences + 1 device int32 that do not decrease),
  * the rows [starts[i], starts[i + 1]) of one batch of `tokens` rows; rows of no sequence get zeros.  (starts are

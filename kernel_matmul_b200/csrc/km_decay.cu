@@ -598,6 +598,7 @@ static int check_problem(const char *name, const km_decay_problem *p) {
                KM_ERR_INVALID_ARGUMENT, "%s: bad element type", name);
     KM_REQUIRE(p->path == 1 || (p->path == 2 && p->dtype != KM_TYPE_F32), KM_ERR_UNSUPPORTED,
                "%s: path must be 1 (FMA pipe) or, for 16-bit types, 2 (tensor cores)", name);
+    KM_REQUIRE(p->reverse >= 0 && p->reverse <= 2, KM_ERR_INVALID_ARGUMENT, "%s: reverse must be 0, 1 or 2", name);
     KM_REQUIRE(p->states >= 0 && p->states <= 2, KM_ERR_INVALID_ARGUMENT, "%s: states must be 0, 1 or 2", name);
     KM_REQUIRE(p->sequences >= 0 && p->tokens >= 0 && p->groups >= 0 && p->group >= 1, KM_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
     KM_REQUIRE(p->dk >= 1 && p->dk <= KM_DECAY_MAX_DIM && p->dv >= 1 && p->dv <= KM_DECAY_MAX_DIM, KM_ERR_UNSUPPORTED,
@@ -688,10 +689,12 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     a.states = static_cast<float *>(workspace);
     a.state_slots = plan.states;
     a.state_row = p.states == 2 ? 1 : (int)p.dv, a.state_col = p.states == 2 ? (int)p.dk : 1;
-    a.scale_in = p.reverse ? p.scale : 1.0f;
-    a.scale_out = p.reverse ? 1.0f : p.scale;
-    a.reverse = p.reverse != 0;
-    a.parts = p.dtype == KM_TYPE_BF16 ? 3 : 2;
+    a.reverse = p.reverse == 1;
+    a.scale_in = a.reverse ? p.scale : 1.0f;
+    a.scale_out = a.reverse ? 1.0f : p.scale;
+    // In bf16 the state, an fp32 result, needs three parts of the decayed keys; forward calls take them whether or not it is asked for, so that
+    // the result is the same.  The passes of a gradient that return no state do with two (2^-17).
+    a.parts = p.dtype == KM_TYPE_BF16 && (p.reverse == 0 || a.state_out.data != nullptr) ? 3 : 2;
     a.wait_polls = current_wait_polls();
     a.gave_up = plan.tc ? gave_up_word() : nullptr;
     KM_REQUIRE(a.slots * a.heads < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_attention: more than 2^31 work items");

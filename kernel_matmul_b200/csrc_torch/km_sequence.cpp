@@ -165,7 +165,7 @@ struct DecayCall {
     int64_t path;
     int32_t type;
 
-    km_decay_problem problem(bool reverse, bool transposed, bool wide) const {
+    km_decay_problem problem(int32_t reverse, bool transposed, bool wide) const {
         km_decay_problem p{};
         p.dtype = type, p.out_dtype = wide ? KM_TYPE_F32 : type;
         p.reverse = reverse, p.path = (int32_t)path;
@@ -215,7 +215,7 @@ struct DecayCall {
     const int32_t *starts_ptr() const { return starts.defined() ? starts.const_data_ptr<int32_t>() : nullptr; }
 
     // `states`: the workspace of a call over the same states with dk and dv swapped (undefined: none).  Returns this call's own.
-    Tensor run(bool reverse, bool transposed, const Tensor &ta, const Tensor &tb, const Tensor &tc, const Tensor &out, const Tensor &state_in,
+    Tensor run(int32_t reverse, bool transposed, const Tensor &ta, const Tensor &tb, const Tensor &tc, const Tensor &out, const Tensor &state_in,
                const Tensor &state_out, const Tensor &states = Tensor()) const {
         const Tensor a = ready(ta), b = ready(tb), c = ready(tc);
         km_decay_problem p = problem(reverse, transposed, out.scalar_type() == at::kFloat);
@@ -240,7 +240,7 @@ struct DecayCall {
         const auto opt = q.options().requires_grad(false);
         const int64_t group = heads / groups;
         Tensor out = at::empty({q.size(0), tokens, heads, dim}, group > 1 ? opt.dtype(at::kFloat) : opt);
-        states = run(true, transposed, a, b, c, out, state_in, state_out, states);
+        states = run(1, transposed, a, b, c, out, state_in, state_out, states);
         if (group == 1) return out;
         Tensor sums = at::empty({q.size(0), tokens, groups, dim}, opt);
         raise_on(km_group_sums(type, q.size(0) * tokens, groups, group, dim, out.const_data_ptr<float>(), sums.data_ptr(), stream_of(q)));
@@ -252,7 +252,7 @@ static variable_list decay_forward(const DecayCall &c, bool return_state, Tensor
     const c10::cuda::CUDAGuard guard(c.q.device());
     poll_gave_up(c.q.device().index());
     Tensor out = c.result_like(), state = return_state ? c.state_like() : Tensor();
-    const Tensor ws = c.run(false, false, c.q, c.k, c.v, out, c.initial, state);
+    const Tensor ws = c.run(0, false, c.q, c.k, c.v, out, c.initial, state);
     if (states != nullptr) *states = ws;
     return return_state ? variable_list{out, state} : variable_list{out};
 }
@@ -285,7 +285,7 @@ struct DecayFunction : torch::autograd::Function<DecayFunction> {
         go = c.ready(go);
         if (ctx->needs_input_grad(0)) {
             out[0] = at::empty({c.q.size(0), c.tokens, c.heads, c.dk}, c.q.options().requires_grad(false));
-            c.run(false, true, go, c.v, c.k, out[0], c.initial, Tensor(), s[6]);
+            c.run(2, true, go, c.v, c.k, out[0], c.initial, Tensor(), s[6]);
         }
         const bool initial = c.initial.defined() && ctx->needs_input_grad(4);
         Tensor back;  // the states of the way back, which the gradients of v and k share
@@ -295,7 +295,7 @@ struct DecayFunction : torch::autograd::Function<DecayFunction> {
         }
         if (ctx->needs_input_grad(1)) out[1] = c.summed(true, c.v, go, c.q, c.dk, ds, Tensor(), back);
         if (ctx->needs_input_grad(3)) {
-            const km_decay_problem p = c.problem(false, false, false);
+            const km_decay_problem p = c.problem(0, false, false);
             out[3] = at::empty({c.heads}, c.log_decay.options().requires_grad(false));
             const size_t bytes = km_decay_gradient_workspace_bytes(&p);
             const Tensor ws = workspace(c.q, bytes);
