@@ -7,94 +7,108 @@ namespace km {
 
 // ------------------------------------------------------------------------------------------------
 // Whole sequences on the FMA pipe: fp32 operands (products of fp32 values have no exact form on the tensor cores), and the
-// other types on path 1.  One CTA of 256 threads per (segment, head); chunks of 32 tokens, so that the products inside a
-// chunk (32 x 32 x (dk + dv)) cost a quarter of those with the state (2 x 32 x dk x dv).  The state is held in registers,
-// 8 x 8 values per thread, for its update, and in shared memory for the product with q.
+// other types on path 1.  Chunks of 32 tokens, so that the products inside a chunk (32 x 32 x (dk + dv)) cost a quarter of those
+// with the state (2 x 32 x dk x dv).  One CTA of 256 threads per (segment, head, 64 columns of v): the state's columns are
+// independent, and two CTAs of half the columns fit an SM where one with all of them did.  The state is held in registers, ROWS x 4
+// values per thread, for its update, and in shared memory for the product with q.  ROWS = 4: for dk up to 64, half of the work.
+// The next chunk's values are on their way while a chunk is worked on.  Forwards and backwards (with decay_gradient_kernel), in us: 2 x 1001
+// tokens, 6 heads of 40 and 72: 246 (all columns in one CTA, one load after the other: 361); 16 x 2048, 16 heads of 64: 3960 (9230);
+// 4 x 4096, 16 heads of 128: 7720 (8930).  Bound by shared memory's bandwidth, of which a product takes 4 to 5 cycles for 4 of FMAs.
 constexpr int FC = 32;          // tokens of a chunk
-constexpr int FLD = 132;        // floats of a row of q, k, v in shared memory
-constexpr int FMA_SMEM = (3 * FC * FLD + FC * 36 + KM_DECAY_MAX_DIM * KM_DECAY_MAX_DIM) * 4;
+constexpr int FV = 64;          // columns of v of a CTA
 
-// Rows [first, first + tokens) of an operand into shared memory, zeros behind them and behind `dim`.  A thread's values are all under
-// way before the first is stored (one after the other they took a chunk 15 us).
-template <typename T, int LD, int WIDTH>
-__device__ __forceinline__ void load_chunk(float *dst, const DecayArgs &a, const Segment &s, const Operand &o, int64_t hg, int64_t hi,
-                                           int first, int tokens, int dim) {
-    constexpr int STEP = 256 / WIDTH, N = FC / STEP;
-    const T *src = o.at<T>(a.starts == nullptr ? s.seq : 0, hg, hi);
-    const int c = threadIdx.x % WIDTH, t0 = threadIdx.x / WIDTH;
-    const T *p = src + token_row(a, s, first + t0) * o.row + c * o.col;
-    const int64_t step = (a.reverse ? -STEP : STEP) * o.row;
-    float x[N];
+// Rows [first, first + tokens) of an operand on the way to shared memory, zeros behind them and behind `dim`.
+template <typename T, int WIDTH>
+struct ChunkRows {
+    static constexpr int STEP = 256 / WIDTH, N = FC / STEP;
+    T x[N];
+    __device__ __forceinline__ void fetch(const DecayArgs &a, const Segment &s, const Operand &o, int64_t hg, int64_t hi, int first, int tokens,
+                                          int dim) {
+        const T *src = o.at<T>(a.starts == nullptr ? s.seq : 0, hg, hi);
+        const int c = threadIdx.x % WIDTH, t0 = threadIdx.x / WIDTH;
+        const T *p = src + token_row(a, s, first + t0) * o.row + c * o.col;
+        const int64_t step = (a.reverse ? -STEP : STEP) * o.row;
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = t0 + i * STEP < tokens && c < dim ? as_float(p[i * step]) : 0.0f;
+        for (int i = 0; i < N; i++) x[i] = t0 + i * STEP < tokens && c < dim ? p[i * step] : from_float<T>(0.0f);
+    }
+    template <int LD>
+    __device__ __forceinline__ void put(float *dst) const {
+        const int c = threadIdx.x % WIDTH, t0 = threadIdx.x / WIDTH;
 #pragma unroll
-    for (int i = 0; i < N; i++) dst[(t0 + i * STEP) * LD + c] = x[i];
-}
+        for (int i = 0; i < N; i++) dst[(t0 + i * STEP) * LD + c] = as_float(x[i]);
+    }
+};
 
-template <typename T, typename O, bool STATE_ONLY>
-__global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
+template <int ROWS>
+struct FmaSmem {
+    static constexpr int LD = 16 * ROWS + 4;
+    static constexpr int Q = 0, K = FC * LD, V = 2 * FC * LD, P = V + FC * (FV + 4), W = P + FC * 36, Z = W + FC, BYTES = (Z + 16 * ROWS * FV) * 4;
+};
+
+template <typename T, typename O, int ROWS, bool STATE_ONLY>
+__global__ void __launch_bounds__(256, 2) decay_fma_kernel(DecayArgs a, int vblocks) {
+    using L = FmaSmem<ROWS>;
+    constexpr int LD = L::LD, LV = FV + 4;
     extern __shared__ __align__(16) float smem[];
-    float *sq = smem, *sk = sq + FC * FLD, *sv = sk + FC * FLD, *sp = sv + FC * FLD, *sz = sp + FC * 36;
-    const int64_t h = blockIdx.x % (unsigned)a.heads, slot = blockIdx.x / (unsigned)a.heads;
+    float *sq = smem + L::Q, *sk = smem + L::K, *sv = smem + L::V, *sp = smem + L::P, *sw = smem + L::W, *sz = smem + L::Z;
+    const int vb = blockIdx.x % (unsigned)vblocks, v0 = vb * FV, cols = min(FV, a.dv - v0);
+    const unsigned rest = blockIdx.x / (unsigned)vblocks;
+    const int64_t h = rest % (unsigned)a.heads, slot = rest / (unsigned)a.heads;
     const int64_t hg = h / a.group, hi = h - hg * a.group;
     const Segment s = find_segment(a, slot);
-    if (!STATE_ONLY && s.spare >= 0) clear_spare_rows<O>(a, s, hg, hi);
+    if (!STATE_ONLY && s.spare >= 0 && vb == 0) clear_spare_rows<O>(a, s, hg, hi);
     if (!s.used || (STATE_ONLY && s.last)) return;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const float g2 = log2_decay(a.log_decay[h]);
     const int dk4 = (a.dk + 3) & ~3;
+    Operand v = a.v;
+    v.data += v0 * v.col * (int64_t)sizeof(T);
 
-    // state: rows ty + 16 i, columns 4 tx + 64 j .. + 3
-    float z[8][8];
+    // state: rows ROWS ty + i, columns 4 tx .. + 3 of this CTA's
+    float z[ROWS][4];
     const bool first_segment = s.first == 0;
+    const float enter = first_segment && !a.reverse && s.length > 0 ? exp2f(g2) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < ROWS; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
+        for (int j = 0; j < 4; j++) {
+            const int r = ROWS * ty + i, c = 4 * tx + j;
             float x = 0.0f;
-            if (!STATE_ONLY && r < a.dk && c < a.dv) {
+            if (!STATE_ONLY && r < a.dk && c < cols) {
                 if (!first_segment)
-                    x = a.states[((int64_t)s.start * a.heads + h) * a.dk * a.dv + r * a.state_row + c * a.state_col];
+                    x = a.states[((int64_t)s.start * a.heads + h) * a.dk * a.dv + r * a.state_row + (v0 + c) * a.state_col];
                 else if (a.state_in.data != nullptr)
-                    x = a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + c * a.state_in.col];
+                    x = a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + (v0 + c) * a.state_in.col] * enter;
             }
             z[i][j] = x;
         }
-    if (!STATE_ONLY && s.length == 0) {  // nothing to go through: the state as it came
-        if (a.state_out.data != nullptr)
-            for (int i = 0; i < 8; i++)
-                for (int j = 0; j < 8; j++) {
-                    const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
-                    if (r < a.dk && c < a.dv) a.state_out.at<float>(s.seq, hg, hi)[r * a.state_out.row + c * a.state_out.col] = z[i][j];
-                }
-        return;
-    }
-    if (!STATE_ONLY && first_segment && !a.reverse) {
-        const float w = exp2f(g2);
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) z[i][j] *= w;
-    }
+    ChunkRows<T, 16 * ROWS> nq, nk;
+    ChunkRows<T, FV> nv;
+    const auto fetch = [&](int first) {
+        const int tokens = min(FC, s.first + s.count - first);
+        if (!STATE_ONLY) nq.fetch(a, s, a.q, hg, hi, first, tokens, a.dk);
+        nk.fetch(a, s, a.k, hg, hi, first, tokens, a.dk);
+        nv.fetch(a, s, v, hg, hi, first, tokens, cols);
+    };
+    if (s.count > 0) fetch(s.first);
 
     for (int first = s.first; first < s.first + s.count; first += FC) {
         const int tokens = min(FC, s.first + s.count - first);
         const bool final = first + tokens == s.length;
         const int e = final && !a.reverse ? tokens - 1 : tokens;
         __syncthreads();
-        if (!STATE_ONLY) load_chunk<T, FLD, 128>(sq, a, s, a.q, hg, hi, first, tokens, a.dk);
-        load_chunk<T, FLD, 128>(sk, a, s, a.k, hg, hi, first, tokens, a.dk);
-        load_chunk<T, FLD, 128>(sv, a, s, a.v, hg, hi, first, tokens, a.dv);
+        if (!STATE_ONLY) nq.template put<LD>(sq);
+        nk.template put<LD>(sk);
+        nv.template put<LV>(sv);
+        if (tid < FC) sw[tid] = exp2f(g2 * (float)max(e - tid, 0)) * a.scale_in;
         if (!STATE_ONLY) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    *reinterpret_cast<float4 *>(sz + (ty + 16 * i) * 128 + 4 * tx + 64 * j) =
-                        make_float4(z[i][4 * j], z[i][4 * j + 1], z[i][4 * j + 2], z[i][4 * j + 3]);
+            for (int i = 0; i < ROWS; i++)
+                *reinterpret_cast<float4 *>(sz + (ROWS * ty + i) * FV + 4 * tx) =
+                    ROWS * ty + i < a.dk ? make_float4(z[i][0], z[i][1], z[i][2], z[i][3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // (not 0 * inf)
         }
         __syncthreads();
+        if (first + FC < s.first + s.count) fetch(first + FC);
         if (!STATE_ONLY) {
             float p[2][2] = {};
 #pragma unroll 2
@@ -102,8 +116,8 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
                 float4 x[2], y[2];
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    x[i] = *reinterpret_cast<const float4 *>(sq + (ty + 16 * i) * FLD + c);
-                    y[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * FLD + c);
+                    x[i] = *reinterpret_cast<const float4 *>(sq + (ty + 16 * i) * LD + c);
+                    y[i] = *reinterpret_cast<const float4 *>(sk + (tx + 16 * i) * LD + c);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; i++)
@@ -123,84 +137,86 @@ __global__ void __launch_bounds__(256) decay_fma_kernel(DecayArgs a) {
                     sp[t * 36 + u] = t >= u ? p[i][j] * exp2f(g2 * (float)(t - u)) * (a.scale_in * a.scale_out) : 0.0f;
                 }
             __syncthreads();
-            float o[2][8] = {};
-#pragma unroll 4
-            for (int c = 0; c < a.dk; c++) {
-                const float4 z0 = *reinterpret_cast<const float4 *>(sz + c * 128 + 4 * tx);
-                const float4 z1 = *reinterpret_cast<const float4 *>(sz + c * 128 + 4 * tx + 64);
+            float o[2][4] = {};
+            const auto add = [&o](int i, float x, const float4 &y) {
+                o[i][0] = fmaf(x, y.x, o[i][0]), o[i][1] = fmaf(x, y.y, o[i][1]);
+                o[i][2] = fmaf(x, y.z, o[i][2]), o[i][3] = fmaf(x, y.w, o[i][3]);
+            };
+#pragma unroll 2
+            for (int c = 0; c < dk4; c += 4) {
+                float4 zz[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) zz[j] = *reinterpret_cast<const float4 *>(sz + (c + j) * FV + 4 * tx);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float x = sq[(ty + 16 * i) * FLD + c];
-                    o[i][0] = fmaf(x, z0.x, o[i][0]), o[i][1] = fmaf(x, z0.y, o[i][1]);
-                    o[i][2] = fmaf(x, z0.z, o[i][2]), o[i][3] = fmaf(x, z0.w, o[i][3]);
-                    o[i][4] = fmaf(x, z1.x, o[i][4]), o[i][5] = fmaf(x, z1.y, o[i][5]);
-                    o[i][6] = fmaf(x, z1.z, o[i][6]), o[i][7] = fmaf(x, z1.w, o[i][7]);
+                    const float4 x = *reinterpret_cast<const float4 *>(sq + (ty + 16 * i) * LD + c);
+                    add(i, x.x, zz[0]), add(i, x.y, zz[1]), add(i, x.z, zz[2]), add(i, x.w, zz[3]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float w = exp2f(g2 * (float)(ty + 16 * i)) * a.scale_out;
 #pragma unroll
-                for (int j = 0; j < 8; j++) o[i][j] *= w;
+                for (int j = 0; j < 4; j++) o[i][j] *= w;
             }
-#pragma unroll 4
-            for (int u = 0; u < tokens; u++) {
-                const float4 v0 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx);
-                const float4 v1 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx + 64);
+#pragma unroll 2
+            for (int u = 0; u < tokens; u += 4) {
+                float4 vv[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) vv[j] = *reinterpret_cast<const float4 *>(sv + (u + j) * LV + 4 * tx);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float x = sp[(ty + 16 * i) * 36 + u];
-                    if (u > ty + 16 * i) continue;  // later tokens do not reach this one, not even as 0 * inf
-                    o[i][0] = fmaf(x, v0.x, o[i][0]), o[i][1] = fmaf(x, v0.y, o[i][1]);
-                    o[i][2] = fmaf(x, v0.z, o[i][2]), o[i][3] = fmaf(x, v0.w, o[i][3]);
-                    o[i][4] = fmaf(x, v1.x, o[i][4]), o[i][5] = fmaf(x, v1.y, o[i][5]);
-                    o[i][6] = fmaf(x, v1.z, o[i][6]), o[i][7] = fmaf(x, v1.w, o[i][7]);
+                    const int t = ty + 16 * i;
+                    const float4 x = *reinterpret_cast<const float4 *>(sp + t * 36 + u);
+                    if (u <= t) add(i, x.x, vv[0]);  // later tokens do not reach this one, not even as 0 * inf
+                    if (u + 1 <= t) add(i, x.y, vv[1]);
+                    if (u + 2 <= t) add(i, x.z, vv[2]);
+                    if (u + 3 <= t) add(i, x.w, vv[3]);
                 }
             }
-            O *out = a.out.at<O>(a.starts == nullptr ? s.seq : 0, hg, hi);
+            O *out = a.out.at<O>(a.starts == nullptr ? s.seq : 0, hg, hi) + v0 * a.out.col;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int t = ty + 16 * i;
                 if (t >= tokens) continue;
                 O *row = out + token_row(a, s, first + t) * a.out.row;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int c = 4 * tx + 64 * (j >> 2) + (j & 3);
-                    if (c < a.dv) row[c * a.out.col] = from_float<O>(o[i][j]);
-                }
+                for (int j = 0; j < 4; j++)
+                    if (4 * tx + j < cols) row[(4 * tx + j) * a.out.col] = from_float<O>(o[i][j]);
             }
         }
         const float carry = exp2f(g2 * (float)e);
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) z[i][j] *= carry;
+            for (int j = 0; j < 4; j++) z[i][j] *= carry;
 #pragma unroll 4
         for (int u = 0; u < tokens; u++) {
-            const float w = exp2f(g2 * (float)(e - u)) * a.scale_in;
-            const float4 v0 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx);
-            const float4 v1 = *reinterpret_cast<const float4 *>(sv + u * FLD + 4 * tx + 64);
+            const float w = sw[u];
+            const float4 vv = *reinterpret_cast<const float4 *>(sv + u * LV + 4 * tx);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float x = sk[u * FLD + ty + 16 * i] * w;
-                z[i][0] = fmaf(x, v0.x, z[i][0]), z[i][1] = fmaf(x, v0.y, z[i][1]);
-                z[i][2] = fmaf(x, v0.z, z[i][2]), z[i][3] = fmaf(x, v0.w, z[i][3]);
-                z[i][4] = fmaf(x, v1.x, z[i][4]), z[i][5] = fmaf(x, v1.y, z[i][5]);
-                z[i][6] = fmaf(x, v1.z, z[i][6]), z[i][7] = fmaf(x, v1.w, z[i][7]);
+            for (int i = 0; i < ROWS; i += 4) {
+                const float4 k4 = *reinterpret_cast<const float4 *>(sk + u * LD + ROWS * ty + i);
+                const float x[4] = {k4.x * w, k4.y * w, k4.z * w, k4.w * w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    z[i + j][0] = fmaf(x[j], vv.x, z[i + j][0]), z[i + j][1] = fmaf(x[j], vv.y, z[i + j][1]);
+                    z[i + j][2] = fmaf(x[j], vv.z, z[i + j][2]), z[i + j][3] = fmaf(x[j], vv.w, z[i + j][3]);
+                }
             }
         }
     }
     if (STATE_ONLY || (s.last && a.state_out.data != nullptr)) {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int r = ty + 16 * i, c = 4 * tx + 64 * (j >> 2) + (j & 3);
-                if (r >= a.dk || c >= a.dv) continue;
+            for (int j = 0; j < 4; j++) {
+                const int r = ROWS * ty + i, c = 4 * tx + j;
+                if (r >= a.dk || c >= cols) continue;
                 if (STATE_ONLY)
-                    a.states[(((int64_t)s.adds * a.heads + h) * a.dk + r) * a.dv + c] = z[i][j];
+                    a.states[(((int64_t)s.adds * a.heads + h) * a.dk + r) * a.dv + v0 + c] = z[i][j];
                 else
-                    a.state_out.at<float>(s.seq, hg, hi)[r * a.state_out.row + c * a.state_out.col] = z[i][j];
+                    a.state_out.at<float>(s.seq, hg, hi)[r * a.state_out.row + (v0 + c) * a.state_out.col] = z[i][j];
             }
     }
 }
@@ -268,13 +284,21 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
 // One CTA per (segment, head, 32 columns of v): the states' columns are independent.  All in fp32, sums over chunks in fp64.
 // STATE_ONLY: the states that a segment adds, from zero (before the scan).
 constexpr int GV = 32;  // columns of v
-constexpr int GRAD_SMEM = (2 * FC * FLD + 2 * FC * 36 + FC * 36 + 2 * KM_DECAY_MAX_DIM * 36) * 4;
 
-template <typename T, bool STATE_ONLY>
-__global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operand dout, Operand dstate, int vblocks, double *partials) {
+// ROWS: groups of 32 rows of the state, 2 for dk up to 64: half of the work, and three CTAs to an SM instead of two.
+template <int ROWS>
+struct GradFmaSmem {
+    static constexpr int LD = 32 * ROWS + 4, LV = GV + 4;
+    static constexpr int Q = 0, K = FC * LD, V = 2 * FC * LD, D = V + FC * LV, W = D + FC * LV, Z = W + 2 * FC, M = Z + 32 * ROWS * LV,
+                         BYTES = (M + 32 * ROWS * LV) * 4;
+};
+
+template <typename T, int ROWS, bool STATE_ONLY>
+__global__ void __launch_bounds__(256, ROWS == 2 ? 3 : 2) decay_gradient_kernel(DecayArgs a, Operand dout, Operand dstate, int vblocks, double *partials) {
+    using L = GradFmaSmem<ROWS>;
+    constexpr int LD = L::LD, LV = L::LV;
     extern __shared__ __align__(16) float smem[];
-    float *sq = smem, *sk = sq + FC * FLD, *sv = sk + FC * FLD, *sd = sv + FC * 36, *sp = sd + FC * 36, *sz = sp + FC * 36,
-          *sm = sz + KM_DECAY_MAX_DIM * 36;
+    float *sq = smem + L::Q, *sk = smem + L::K, *sv = smem + L::V, *sd = smem + L::D, *sw = smem + L::W, *sz = smem + L::Z, *sm = smem + L::M;
     const int vb = blockIdx.x % vblocks;
     const unsigned rest = blockIdx.x / (unsigned)vblocks;
     const int64_t h = rest % a.heads, slot = rest / a.heads;
@@ -294,9 +318,9 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
     // Z, then M, where sequences are cut
     float *own = a.states + ((int64_t)s.adds * a.heads + h) * 2 * state + vb * GV;
     const float *start = a.states + ((int64_t)s.start * a.heads + h) * 2 * state + vb * GV;
-    float z[4][4], m[4][4];
+    float z[ROWS][4], m[ROWS][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < ROWS; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int r = ty + 32 * i, c = 4 * tx + j;
@@ -308,36 +332,55 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
                 z[i][j] = m[i][j] = exp2f(g2) * a.state_in.at<float>(s.seq, hg, hi)[r * a.state_in.row + (vb * GV + c) * a.state_in.col];
         }
     double total = 0.0;
+    ChunkRows<T, 32 * ROWS> nq, nk;
+    ChunkRows<T, GV> nv, nd;
+    const auto fetch = [&](int first) {
+        const int tokens = min(FC, s.first + s.count - first);
+        if (!STATE_ONLY) nq.fetch(a, s, a.q, hg, hi, first, tokens, a.dk);
+        nk.fetch(a, s, a.k, hg, hi, first, tokens, a.dk);
+        nv.fetch(a, s, v, hg, hi, first, tokens, cols);
+        if (!STATE_ONLY) nd.fetch(a, s, d, hg, hi, first, tokens, cols);
+    };
+    if (s.count > 0) fetch(s.first);
     for (int first = s.first; first < s.first + s.count; first += FC) {
         const int tokens = min(FC, s.first + s.count - first);
         const int e = first + tokens == s.length ? tokens - 1 : tokens;
         __syncthreads();
-        if (!STATE_ONLY) load_chunk<T, FLD, 128>(sq, a, s, a.q, hg, hi, first, tokens, a.dk);
-        load_chunk<T, FLD, 128>(sk, a, s, a.k, hg, hi, first, tokens, a.dk);
-        load_chunk<T, 36, GV>(sv, a, s, v, hg, hi, first, tokens, cols);
-        if (!STATE_ONLY) load_chunk<T, 36, GV>(sd, a, s, d, hg, hi, first, tokens, cols);
+        if (!STATE_ONLY) nq.template put<LD>(sq);
+        nk.template put<LD>(sk);
+        nv.template put<LV>(sv);
+        if (!STATE_ONLY) nd.template put<LV>(sd);
+        if (tid < FC) {
+            const float w = exp2f(g2 * (float)max(e - tid, 0));
+            sw[2 * tid] = w, sw[2 * tid + 1] = w * (float)max(e - tid, 0);
+        }
+        if (!STATE_ONLY) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            *reinterpret_cast<float4 *>(sz + (ty + 32 * i) * 36 + 4 * tx) = make_float4(z[i][0], z[i][1], z[i][2], z[i][3]);
-            *reinterpret_cast<float4 *>(sm + (ty + 32 * i) * 36 + 4 * tx) = make_float4(m[i][0], m[i][1], m[i][2], m[i][3]);
+            for (int i = 0; i < ROWS; i++) {
+                const bool row = ty + 32 * i < a.dk;  // (zeros behind dk: not 0 * inf)
+                const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                *reinterpret_cast<float4 *>(sz + (ty + 32 * i) * LV + 4 * tx) = row ? make_float4(z[i][0], z[i][1], z[i][2], z[i][3]) : none;
+                *reinterpret_cast<float4 *>(sm + (ty + 32 * i) * LV + 4 * tx) = row ? make_float4(m[i][0], m[i][1], m[i][2], m[i][3]) : none;
+            }
         }
         __syncthreads();
+        if (first + FC < s.first + s.count) fetch(first + FC);
         float sum = 0.0f;
         if (!STATE_ONLY) {  // inside the chunk: entries (t, u) with t = ty, u = tx + 8 i
             float p[4] = {}, r[4] = {};
             for (int c = 0; c < dk4; c += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(sq + ty * FLD + c);
+                const float4 x = *reinterpret_cast<const float4 *>(sq + ty * LD + c);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 y = *reinterpret_cast<const float4 *>(sk + (tx + 8 * i) * FLD + c);
+                    const float4 y = *reinterpret_cast<const float4 *>(sk + (tx + 8 * i) * LD + c);
                     p[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, p[i]))));
                 }
             }
             for (int c = 0; c < GV; c += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(sd + ty * 36 + c);
+                const float4 x = *reinterpret_cast<const float4 *>(sd + ty * LV + c);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float4 y = *reinterpret_cast<const float4 *>(sv + (tx + 8 * i) * 36 + c);
+                    const float4 y = *reinterpret_cast<const float4 *>(sv + (tx + 8 * i) * LV + c);
                     r[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, r[i]))));
                 }
             }
@@ -349,24 +392,29 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
         }
         if (!STATE_ONLY) {  // from the states: row t = ty, columns 4 tx ..
             float x[4] = {}, y[4] = {};
-#pragma unroll 4
-            for (int c = 0; c < a.dk; c++) {
-                const float qv = sq[ty * FLD + c];
-                const float4 zz = *reinterpret_cast<const float4 *>(sz + c * 36 + 4 * tx);
-                const float4 mm = *reinterpret_cast<const float4 *>(sm + c * 36 + 4 * tx);
-                x[0] = fmaf(qv, zz.x, x[0]), x[1] = fmaf(qv, zz.y, x[1]), x[2] = fmaf(qv, zz.z, x[2]), x[3] = fmaf(qv, zz.w, x[3]);
-                y[0] = fmaf(qv, mm.x, y[0]), y[1] = fmaf(qv, mm.y, y[1]), y[2] = fmaf(qv, mm.z, y[2]), y[3] = fmaf(qv, mm.w, y[3]);
+            const auto add = [](float f, const float4 &v, float (&to)[4]) {
+                to[0] = fmaf(f, v.x, to[0]), to[1] = fmaf(f, v.y, to[1]), to[2] = fmaf(f, v.z, to[2]), to[3] = fmaf(f, v.w, to[3]);
+            };
+#pragma unroll 2
+            for (int c = 0; c < dk4; c += 4) {
+                const float4 qv = *reinterpret_cast<const float4 *>(sq + ty * LD + c);
+                const float f[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    add(f[j], *reinterpret_cast<const float4 *>(sz + (c + j) * LV + 4 * tx), x);
+                    add(f[j], *reinterpret_cast<const float4 *>(sm + (c + j) * LV + 4 * tx), y);
+                }
             }
             const float w = exp2f(g2 * (float)ty);
             float part = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) part = fmaf(fmaf((float)ty, x[j], y[j]), sd[ty * 36 + 4 * tx + j], part);
+            for (int j = 0; j < 4; j++) part = fmaf(fmaf((float)ty, x[j], y[j]), sd[ty * LV + 4 * tx + j], part);
             if (ty < tokens) sum = fmaf(w, part, sum);
         }
         total += (double)sum * (double)a.scale_out;
         const float carry = exp2f(g2 * (float)e);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 m[i][j] = carry * fmaf((float)e, z[i][j], m[i][j]);
@@ -374,11 +422,11 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
             }
 #pragma unroll 4
         for (int u = 0; u < tokens; u++) {
-            const float w = exp2f(g2 * (float)(e - u)), wm = w * (float)(e - u);
-            const float4 vv = *reinterpret_cast<const float4 *>(sv + u * 36 + 4 * tx);
+            const float2 w = *reinterpret_cast<const float2 *>(sw + 2 * u);
+            const float4 vv = *reinterpret_cast<const float4 *>(sv + u * LV + 4 * tx);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float kk = sk[u * FLD + ty + 32 * i], x = kk * w, y = kk * wm;
+            for (int i = 0; i < ROWS; i++) {
+                const float kk = sk[u * LD + ty + 32 * i], x = kk * w.x, y = kk * w.y;
                 z[i][0] = fmaf(x, vv.x, z[i][0]), z[i][1] = fmaf(x, vv.y, z[i][1]), z[i][2] = fmaf(x, vv.z, z[i][2]),
                 z[i][3] = fmaf(x, vv.w, z[i][3]);
                 m[i][0] = fmaf(y, vv.x, m[i][0]), m[i][1] = fmaf(y, vv.y, m[i][1]), m[i][2] = fmaf(y, vv.z, m[i][2]),
@@ -388,7 +436,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
     }
     if (STATE_ONLY) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int r = ty + 32 * i, c = 4 * tx + j;
@@ -398,7 +446,7 @@ __global__ void __launch_bounds__(256) decay_gradient_kernel(DecayArgs a, Operan
     }
     if (dstate.data != nullptr && s.last && s.length > 0) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int r = ty + 32 * i, c = 4 * tx + j;
@@ -626,10 +674,14 @@ static int launch_scan(const DecayArgs &a, cudaStream_t s) {
 
 template <typename T, typename O>
 static int launch_fma(const DecayArgs &a, bool state_only, cudaStream_t s) {
-    auto kernel = state_only ? decay_fma_kernel<T, O, true> : decay_fma_kernel<T, O, false>;
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FMA_SMEM);
+    const bool few = a.dk <= 64;
+    auto kernel = few ? state_only ? decay_fma_kernel<T, O, 4, true> : decay_fma_kernel<T, O, 4, false>
+                      : state_only ? decay_fma_kernel<T, O, 8, true> : decay_fma_kernel<T, O, 8, false>;
+    const int bytes = few ? FmaSmem<4>::BYTES : FmaSmem<8>::BYTES, vblocks = (int)ceil_div(a.dv, FV);
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return cuda_fail(err, "decay_fma_kernel");
-    kernel<<<(unsigned)(a.slots * a.heads), 256, FMA_SMEM, s>>>(a);
+    KM_REQUIRE(a.slots * a.heads * vblocks < (1LL << 31), KM_ERR_UNSUPPORTED, "km_decay_attention: more than 2^31 work items");
+    kernel<<<(unsigned)(a.slots * a.heads * vblocks), 256, bytes, s>>>(a, vblocks);
     KM_CHECK_LAUNCH("decay_fma_kernel launch");
     return KM_OK;
 }
@@ -720,11 +772,12 @@ static size_t grad_states(const km_decay_problem &p) {
 
 template <typename T, bool STATE_ONLY>
 static int launch_grad_fma(const DecayArgs &a, const Operand &d, const Operand &ds, double *partials, cudaStream_t s) {
-    auto kernel = decay_gradient_kernel<T, STATE_ONLY>;
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM);
+    auto kernel = a.dk <= 64 ? decay_gradient_kernel<T, 2, STATE_ONLY> : decay_gradient_kernel<T, 4, STATE_ONLY>;
+    const int bytes = a.dk <= 64 ? GradFmaSmem<2>::BYTES : GradFmaSmem<4>::BYTES;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (err != cudaSuccess) return cuda_fail(err, "decay_gradient_kernel");
     const int vblocks = (int)ceil_div(a.dv, GV);
-    kernel<<<(unsigned)(a.slots * a.heads * vblocks), 256, GRAD_SMEM, s>>>(a, d, ds, vblocks, partials);
+    kernel<<<(unsigned)(a.slots * a.heads * vblocks), 256, bytes, s>>>(a, d, ds, vblocks, partials);
     KM_CHECK_LAUNCH("decay_gradient_kernel launch");
     return KM_OK;
 }
