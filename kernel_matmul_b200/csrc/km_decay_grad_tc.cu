@@ -10,6 +10,9 @@
 // (the products of the states with q and then dO are sums over the tokens first, so that neither state is an operand).
 // Fourteen products of 128^3 with the three parts, 7200 cycles of the tensor pipe per chunk of a head with dk = dv = 128, and between
 // them the parts have to be written into the only three tiles that Q, K, V and dO leave: the phases follow one another.
+// (The products of half of the tokens under the writing of the other half's parts took 706 instead of 728 us for a training step of
+// 4 x 4096 tokens with 16 heads, but small parts then come onto large sums, of which the tensor cores cut the last bits: an error of 5.9e-7 of
+// the gradient for 2.2e-7.)
 #include "km_decay_tc.cuh"
 
 namespace km {

@@ -60,9 +60,9 @@ struct Control {
 // tensor memory columns
 constexpr uint32_t COL_S = 0, COL_PV = 128, COL_QZ = 256, COL_U = 384;
 
-// 2^n that brings a largest magnitude of (biased) exponent e to [2^13, 2^14) (fp16's range and as many of its small values as possible); 1 for 0 and
-// for what is not finite
 __device__ __forceinline__ int exponent_of(float m) { return (int)((__float_as_uint(m) >> 23) & 0xffu); }
+// 2^n that brings a largest magnitude of (biased) exponent e to [2^13, 2^14) (fp16's range and as many of its small values as
+// possible); 1 for 0 and for what is not finite
 __device__ __forceinline__ float fp16_scale(int e) {
     if (e == 0 || e == 255) return 1.0f;
     return __uint_as_float((uint32_t)min(max(127 + 13 - (e - 127), 2), 252) << 23);  // (its inverse is a normal number too)
@@ -274,7 +274,6 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
         bool ok = true;
         for (int it = 0; it < chunks; it++) {
             const int b = it & 1, tokens = min(TC, s.count - it * TC);
-            const int e = s.first + it * TC + tokens == s.length && !a.reverse ? tokens - 1 : tokens;
             ok = mbar_wait_warp(&ctl.full[b], (it >> 1) & 1, a.wait_polls);
             if (!ok) break;
             if (tokens < TC) {  // what lies behind the chunk may be another sequence's: not even 0 * inf may come in

@@ -177,7 +177,7 @@ struct DecayCall {
     }
     // An operand of the tensor-core kernels, which load rows that start on boundaries of 16 bytes by TMA and any others value by
     // value: those are copied into such rows first, but for sequences of a few tokens (4 heads of 33 and 77: 500 tokens take
-    // 159 us without the copies and 48 with them, 64 tokens 46 and 36; a token's three copies cost 10 us of host time).
+    // 159 us without the copies and 49 with them, 64 tokens 46 and 45; a token's three copies cost 10 us of host time).
     Tensor ready(const Tensor &t) const {
         if (type == KM_TYPE_F32 || path == PATH_FMA || t.size(1) < 16) return t;
         bool aligned = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;

@@ -55,3 +55,21 @@ def test_rotary_frequencies():
     assert torch.equal(p[turns >= 32], full[turns >= 32]) and torch.allclose(p[turns <= 1], full[turns <= 1] / 8, rtol=1e-15)
     assert s == 0.1 * math.log(8.0) + 1.0
     assert ops.rotary_frequencies(0, device="cpu")[0].shape == (0,)
+
+
+@pytest.mark.parametrize("field, value", [("reverse", 3), ("reverse", -1), ("states", 3), ("path", 3), ("dk", 0), ("dv", 129), ("group", 0),
+                                          ("tokens", -1), ("tokens", 2**31), ("dtype", 9), ("out_dtype", 2)])
+def test_bad_problems_are_refused(field, value):
+    import ctypes
+
+    from kernel_matmul_b200._lib import KmDecayProblem, lib
+
+    good = dict(dtype=0, out_dtype=0, reverse=0, path=0, sequences=1, tokens=8, groups=2, group=1, dk=16, dv=16, packed=0, states=0, scale=1.0)
+    p = KmDecayProblem(**{**good, field: value})
+    calls = [lambda q: lib.km_decay_attention(q, *[None] * 4, None, None, None, None, None, 0, None),
+             lambda q: lib.km_decay_gradient(q, *[None] * 4, None, None, None, None, None, None, 0, None)]
+    for call in calls:
+        assert call(KmDecayProblem(**good)) != 0 and b"null argument" in lib.km_last_error()
+        assert call(p) != 0 and b"null" not in lib.km_last_error()
+        assert call(ctypes.POINTER(KmDecayProblem)()) != 0 and b"null problem" in lib.km_last_error()
+    assert lib.km_decay_attention_workspace_bytes(p) == 0

@@ -215,6 +215,18 @@ def test_values_that_are_not_finite_stay_in_their_sequence():
             assert torch.isnan(got[150:200, 1]).any()
 
 
+@pytest.mark.parametrize("dk, dv", [(5, 6), (63, 70), (67, 63), (126, 127)])
+def test_an_infinite_value_reaches_its_column_of_later_tokens(dk, dv):
+    """With positive q and k every sum is +inf from that token on and finite elsewhere: nothing behind dk meets it as 0 * inf."""
+    n, at, col = 150, 40, dv - 1
+    q, k = (torch.rand(n, 2, dk, device=DEV) + 0.1 for _ in range(2))
+    v = randn(n, 2, dv)
+    v[at, :, col] = math.inf
+    o, s = ops.decay_attention(q, k, v, torch.full((2,), -0.125, device=DEV), sequence_starts=starts_of([n]), return_state=True)
+    assert torch.isposinf(o[at:, :, col]).all() and o[:at].isfinite().all() and o[:, :, :col].isfinite().all()
+    assert torch.isposinf(s[..., col]).all() and s[..., :col].isfinite().all()
+
+
 def test_sequence_starts_out_of_range_are_clamped():
     q, k, v = (randn(100, 1, 8) for _ in range(3))
     g = decays(1)
