@@ -12,7 +12,7 @@
 // Roundings to 16 bits.  The state's copy in QZ is rounded once, half a step of the operands' type (its low part has no room in
 // shared memory): the only one, besides the result's own, and as large as that.  P goes in two parts (one part made results of
 // short sequences 1.4 - 1.6 times as wrong as their rounding).  Z itself and U stay in fp32 and are fp32 results: K~ goes in two
-// parts in fp16 (2^-22) and three in bf16 (2^-25).  The tensor cores cut the last bits of a sum off at every step of 16 tokens,
+// parts in fp16 (2^-22) and three in bf16 (2^-25; two, 2^-17, in the passes of a gradient that return no state).  The tensor cores cut the last bits of a sum off at every step of 16 tokens,
 // so small parts are added up first: final states are within 1.5e-7 (2-norm, as an fp32 evaluation is) instead of 5e-7, and
 // 2.4e-6 with two parts of bf16.  fp16 has too few exponents for P and Z: both are scaled by powers of two per row, taken back in
 // fp32.
