@@ -122,6 +122,28 @@ def test_attention_gradients(case, dtype):
             assert not got["dq"][:, -case["tail"] :].any() and not got["dv"][:, -case["tail"] :].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [CASES[3], CASES[4], CASES[7], CASES[12], dict(batch=1, tokens=700, heads=2, groups=2, dk=65, dv=65)],
+                         ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_attention_gradients_without_states(case, dtype):
+    """No state comes in and none is asked for: the passes of the gradient return 16-bit results alone."""
+    for path in paths(dtype):
+        x, packed, tokens, _ = make(case, dtype)
+        if case.get("decay") == "mixed":
+            x["log_decay"][0] = -30.0
+        x["initial"].zero_()
+        go = randn(*x["q"].shape[:3], case["dv"], dtype=dtype)
+        leaves = [x[n].requires_grad_() for n in ("q", "k", "v", "log_decay")]
+        q, k, v = (t[0] if packed else t for t in leaves[:3])
+        o = ops.decay_attention(q, k, v, leaves[3], sequence_starts=starts_of(case["lengths"]) if packed else None, path=path)
+        grads = torch.autograd.grad(o, leaves, go[0] if packed else go)
+        if packed and case["tail"]:
+            go[:, -case["tail"] :] = 0
+        want = attention_with_scales({n: t.detach().double() for n, t in x.items()}, case["dk"] ** -0.5, case.get("lengths"),
+                                     [go.double(), torch.zeros_like(x["initial"]).double()])
+        compare({"dq": grads[0], "dk": grads[1], "dv": grads[2], "dlog_decay": grads[3]}, want, None, dtype, case, tokens)
+
+
 def test_attention_gradient_against_differences():
     """Central differences of the fp64 reference are no check of the op, so the op itself is differenced, in fp32: a loss that is
     linear in the op's results; step h = 2^-6, errors h^2 / 6 of third derivatives and 2^-24 sum|terms| / h."""
