@@ -285,7 +285,9 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 ok = mbar_wait_warp(&ctl.s_full, it & 1, a.wait_polls);
                 if (!ok) break;
                 tc_fence_after();
-                // Blocks of 32 rows x 16 columns: `side` < 0 for those before the diagonal in time (all of which count), 0 on it.
+                // Blocks of 32 rows x 16 columns: `side` < 0 for those before the diagonal in time (all of which count), 0 on it.  In the
+                // reverse form the columns from `tokens` on, rows of the tensors behind the sequence, are on that side too: `live` of
+                // a block's columns are this chunk's, and the others, which may hold anything, are no part of the row.
                 // (The loops of this kernel are not unrolled further than registers demand: three kinds of warps run their code
                 // at once, and unrolled it did not fit the instruction cache.)
                 float up = 1.0f;
@@ -293,13 +295,14 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                     float m = 0.0f;
 #pragma unroll 1
                     for (int c0 = half * 16; c0 < TC; c0 += 32) {
-                        const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
-                        if (side > 0) continue;
+                        const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0, live = a.reverse ? tokens - c0 : 16;
+                        if (side > 0 || live <= 0) continue;
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
                         tmem_ld_wait16(r);
 #pragma unroll
-                        for (int j = 0; j < 16; j++) m = fmaxf(m, side < 0 || (a.reverse ? j >= d : j <= d) ? fabsf(__uint_as_float(r[j])) : 0.0f);
+                        for (int j = 0; j < 16; j++)
+                            m = fmaxf(m, (side < 0 || (a.reverse ? j >= d : j <= d)) && j < live ? fabsf(__uint_as_float(r[j])) : 0.0f);
                     }
                     ctl.row_max[1][half][row] = (uint8_t)exponent_of(m);
                     ok = meet();
@@ -309,15 +312,15 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 }
 #pragma unroll 1
                 for (int c0 = half * 16; c0 < TC; c0 += 32) {
-                    const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0;
+                    const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0, live = a.reverse ? tokens - c0 : 16;
                     uint32_t w[16];  // eight words of high parts, eight of low ones
-                    if (side > 0) {
+                    if (side > 0 || live <= 0) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) w[j] = 0;
                     } else {
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
-                        if (side < 0) {
+                        if (side < 0 && live >= 16) {
                             // decay = 2^(g2 (distance to the block's nearer edge)) 2^(g2 (inside the block)), both at most one
                             const f32x2 outer = splat2(ex2_approx(g2 * (float)(a.reverse ? -d : d - 15)) * up);
                             tmem_ld_wait16(r);
@@ -336,8 +339,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                                 const f32x2 x = ex2_approx2(mul2(g22, sub2(d2, pack2((float)(2 * j), (float)(2 * j + 1)))));
                                 float u, v;
                                 unpack2(mul2(HALF ? mul2(x, up2) : x, pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))), u, v);
-                                two_parts<T>((a.reverse ? 2 * j >= d : 2 * j <= d) ? u : 0.0f, (a.reverse ? 2 * j + 1 >= d : 2 * j + 1 <= d) ? v : 0.0f,
-                                             w[j], w[j + 8]);
+                                two_parts<T>((a.reverse ? 2 * j >= d : 2 * j <= d) && 2 * j < live ? u : 0.0f,
+                                             (a.reverse ? 2 * j + 1 >= d : 2 * j + 1 <= d) && 2 * j + 1 < live ? v : 0.0f, w[j], w[j + 8]);
                             }
                         }
                     }
