@@ -502,6 +502,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
             // took them 3000 cycles).  The rows around a sequence's end and what has no map do take that way.
             const float fp = HALF ? intra * __bfloat162float(ctl.p_scale[it & 1][row]) : intra;
             unsigned char *box = smem + b * L::STAGE + L::Q + warp * 4096;
+            const int r0 = (warp & 3) * 32, to_row = chunk_row(a, s, it, tokens);
+            const bool by_map = maps.use[3] && r0 + 32 <= tokens;
             static_assert(L::K >= 8 * 4096, "a box for each warp");
 #pragma unroll
             for (int round = 0; round < NO / CB; round++) {
@@ -536,8 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                         *reinterpret_cast<uint4 *>(box + swizzled<PITCH>(lane * PITCH + (cb / VALUES + j) * 16)) =
                             make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 }
-                const int r0 = (warp & 3) * 32, x0 = half * NO + round * CB, to_row = chunk_row(a, s, it, tokens);
-                const bool by_map = maps.use[3] && r0 + 32 <= tokens;
+                const int x0 = half * NO + round * CB;
                 if (by_map) fence_async_smem();
                 if (round == NO / CB - 1) {
                     tc_fence_before();
@@ -569,6 +570,9 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                     }
                 }
             }
+            // The next copy into this tile is TMA's: it has to come after what the threads wrote and read here.  (Results that went by a
+            // map are behind such a fence already.)
+            if (!by_map) fence_async_smem();
             mbar_arrive(&ctl.q_empty[b]);
         }
         if (row < a.dv && (STATE_ONLY || (s.last && a.state_out.data != nullptr))) {
