@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                                                                         const __grid_constant__ Operand dstate,
                                                                         const __grid_constant__ GradMaps maps, double *partials) {
     using L = GradSmem<KB, VB>;
-    constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    constexpr int PARTS = HALF ? 2 : 3;
     constexpr int NZ = KB * 16;  // of the states' rows: this thread's columns
     constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
     extern __shared__ unsigned char raw[];
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
     }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = (s.count + TC - 1) / TC;
     const float g2 = log2_decay(a.log_decay[h]);
+    const bool grows = HALF && g2 > 0.0f;
     if (tid == 0) {
         mbar_init(&ctl.full, 33), mbar_init(&ctl.sg_full, 1), mbar_init(&ctl.done, 1), mbar_init(&ctl.drain, 1);
         mbar_init(&ctl.ready, ARITH), mbar_init(&ctl.read, ARITH);
@@ -232,8 +234,9 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                 fence_async_smem();
                 mbar_arrive(&ctl.ready);
             };
-            const auto before_last = [&](int t) { return exp2f(g2 * (float)max(last - t, 0)); };
-            const auto behind_first = [&](int t) { return exp2f(g2 * (float)t); };
+            // (what grows in fp16 is taken relative to the largest, and the rest in fp32)
+            const auto before_last = [&](int t) { return exp2f(g2 * (float)(max(last - t, 0) - (grows ? last : 0))); };
+            const auto behind_first = [&](int t) { return exp2f(g2 * (float)(grows ? t - last : t)); };
             parts(L::K, before_last);
             // (under the products U)
             f32x2 sum = splat2(0.0f);
@@ -285,7 +288,8 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             }
             tc_fence_after();
             const f32x2 carry = splat2(exp2f(g2 * (float)e)), steps = splat2((float)e), whole = splat2(1.0f / PART);
-            const f32x2 beyond = splat2(exp2f(g2 * (float)(e - last)));
+            const f32x2 beyond = splat2(exp2f(g2 * (float)(grows ? e : e - last)));
+            const f32x2 back = splat2(grows ? exp2f(g2 * (float)last) : 1.0f);  // of X and X'
 #pragma unroll
             for (int c = 0; c < NZ; c += 8) {
                 uint32_t x[8], x1[8], u[8], u1[8];
@@ -302,8 +306,9 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                     f32x2 &zz = z[c / 2 + j], &mm = m[c / 2 + j];
                     const auto pair = [](const uint32_t &p, const uint32_t &q) { return pack2(__uint_as_float(p), __uint_as_float(q)); };
                     if (!STATE_ONLY && state_row) {  // (VB = 1: the other lanes repeat these)
-                        sum = fma2(pair(x[2 * j], x[2 * j + 1]), mm, sum);
-                        sum = fma2(mul2(whole, pair(x1[2 * j], x1[2 * j + 1])), zz, sum);
+                        const f32x2 p = pair(x[2 * j], x[2 * j + 1]), p1 = mul2(whole, pair(x1[2 * j], x1[2 * j + 1]));
+                        sum = fma2(HALF ? mul2(back, p) : p, mm, sum);
+                        sum = fma2(HALF ? mul2(back, p1) : p1, zz, sum);
                     }
                     mm = fma2(carry, fma2(steps, zz, mm), mul2(beyond, mul2(whole, pair(u1[2 * j], u1[2 * j + 1]))));
                     zz = fma2(carry, zz, mul2(beyond, pair(u[2 * j], u[2 * j + 1])));

@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const float g2 = log2_decay(a.log_decay[h]);
+    const bool grows = HALF && g2 > 0.0f;  // (bf16 has the exponents of fp32)
     if (warp == MMA_WARP) tmem_alloc(&ctl.tmem, 512);
     if (warp == MMA_WARP + 1 && lane < 16) ctl.inner[lane] = exp2f(g2 * (float)(a.reverse ? lane : 15 - lane));
     tc_fence_before();
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 // (The loops of this kernel are not unrolled further than registers demand: three kinds of warps run their code
                 // at once, and unrolled it did not fit the instruction cache.)
                 float up = 1.0f;
-                if (HALF) {  // scaling from the largest of the row's products: decays only make them smaller
+                if (HALF) {  // scaling from the largest of the row's products, times what a block's can grow by at most (decays only make them smaller)
                     float m = 0.0f;
 #pragma unroll 1
                     for (int c0 = half * 16; c0 < TC; c0 += 32) {
@@ -300,9 +301,12 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
                         tmem_ld_wait16(r);
+                        float largest = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 16; j++)
-                            m = fmaxf(m, (side < 0 || (a.reverse ? j >= d : j <= d)) && j < live ? fabsf(__uint_as_float(r[j])) : 0.0f);
+                            largest = fmaxf(largest, (side < 0 || (a.reverse ? j >= d : j <= d)) && j < live ? fabsf(__uint_as_float(r[j])) : 0.0f);
+                        if (grows) largest *= ex2_approx(g2 * (float)max(a.reverse ? 15 - d : d, 0));  // (its farthest column)
+                        m = fmaxf(m, largest);
                     }
                     ctl.row_max[1][half][row] = (uint8_t)exponent_of(m);
                     ok = meet();
@@ -321,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
                         if (side < 0 && live >= 16) {
-                            // decay = 2^(g2 (distance to the block's nearer edge)) 2^(g2 (inside the block)), both at most one
+                            // decay = 2^(g2 (distance to the block's nearer edge)) 2^(g2 (inside the block))
                             const f32x2 outer = splat2(ex2_approx(g2 * (float)(a.reverse ? -d : d - 15)) * up);
                             tmem_ld_wait16(r);
 #pragma unroll
@@ -363,7 +367,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 const int m = (mine >> 3) + 32 * (i & 3);
                 // (rows behind the last token are zero, whatever is in them)
                 if (m >= tokens) x = make_uint4(0, 0, 0, 0);
-                const f32x2 w = splat2(exp2f(g2 * (float)max(a.reverse ? m : tokens - 1 - m, 0)));  // decay to the chunk's last token
+                // decay to the chunk's last token; where it grows in fp16, relative to that of the chunk's first
+                const f32x2 w = splat2(exp2f(g2 * (float)(max(a.reverse ? m : tokens - 1 - m, 0) - (grows ? tokens - 1 : 0))));
                 const uint32_t in[4] = {x.x, x.y, x.z, x.w};
                 uint32_t high[4], low[4], lowest[4];
 #pragma unroll
@@ -473,8 +478,9 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
-            // (K~ is decayed to the chunk's last token, which keeps its largest entries in fp16's range; the step beyond it is taken here)
-            const f32x2 carry2 = splat2(carry), in2 = splat2(a.scale_in * exp2f(g2 * (float)(e - tokens + 1)));
+            // (K~ is decayed to the chunk's last token, which keeps its largest entries in fp16's range; the step beyond it, and those that growing
+            // keys are short of, are taken here)
+            const f32x2 carry2 = splat2(carry), in2 = splat2(a.scale_in * exp2f(g2 * (float)(grows ? e : e - tokens + 1)));
 #pragma unroll
             for (int cb = 0; cb < NZ / 16; cb++) {
                 uint32_t r[16];
