@@ -2,7 +2,7 @@
 // state): 16-bit operands, chunks of 128 tokens, one CTA per (sequence, head).
 //
 // The gradient is an fp32 sum, so nothing of it may be rounded to 16 bits but the decayed operands, which go in parts: two in fp16
-// (2^-22), three in bf16 (2^-25).  Per chunk, with d = t - s, e the exponent of the chunk's end and all accumulators fp32:
+// (2^-22, scaled by powers of two to the top of its range: 2^-39 of a chunk's largest), three in bf16 (2^-25).  Per chunk, with d = t - s, e the exponent of the chunk's end and all accumulators fp32:
 //   S = Q K^T, G = dO V^T:  sum over s < t of d e^{g d} S G, entry by entry in registers
 //   U  = V^T K~, U' = V^T K':       K~ = e^{g (e - s)} K,  K' = (e - s) e^{g (e - s)} K
 //   X  = dO^T Q~, X' = dO^T Q':     Q~ = e^{g t} Q,        Q' = t e^{g t} Q
@@ -29,11 +29,12 @@ struct GradMaps {
 };
 
 struct GradControl {
-    uint64_t full, sg_full, ready, done, read, drain;
+    uint64_t full, sg_full, ready, done, read, drain, meet;
     uint32_t tmem;
     int dead;
     float inner[16];  // 2^(g2 (15 - j))
     double sums[ARITH / 32];
+    alignas(16) uint16_t largest[2][2][ARITH / 32];  // fp16: magnitudes of K and Q that a warp has seen, as bits, by parity of the chunk
 };
 
 template <int KB, int VB>
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
     const bool grows = HALF && g2 > 0.0f;
     if (tid == 0) {
         mbar_init(&ctl.full, 33), mbar_init(&ctl.sg_full, 1), mbar_init(&ctl.done, 1), mbar_init(&ctl.drain, 1);
-        mbar_init(&ctl.ready, ARITH), mbar_init(&ctl.read, ARITH);
+        mbar_init(&ctl.ready, ARITH), mbar_init(&ctl.read, ARITH), mbar_init(&ctl.meet, ARITH);
         ctl.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -222,14 +223,36 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             if (tokens < TC)  // rows behind the chunk may be another sequence's: not even 0 * inf may come in
                 for (int p = tid; p < (STATE_ONLY ? 1 : 2) * VB * TC * 8; p += ARITH)
                     if (((p >> 3) & (TC - 1)) >= tokens) *reinterpret_cast<uint4 *>(smem + L::V + p * 16) = make_uint4(0, 0, 0, 0);
+            // fp16: K~, K', Q~ and Q' are scaled by the chunk's largest key and query: values below fp16's normal range would leave
+            // their low parts no bits
+            const auto up = [&](int which) {
+                if constexpr (!HALF) return 1.0f;
+                static_assert(ARITH / 32 == 16, "two loads");
+                const uint4 *m = reinterpret_cast<const uint4 *>(ctl.largest[it & 1][which]);
+                return fp16_scale_of_bits(fp16_larger(fp16_largest(fp16_largest(0, m[0]), m[1])));
+            };
+            if (HALF) {
+#pragma unroll
+                for (int which = 0; which < (STATE_ONLY ? 1 : 2); which++) {
+                    uint32_t m = 0;
+                    for (int p = tid; p < KB * TC * 8; p += ARITH)
+                        if (((p >> 3) & (TC - 1)) < tokens) m = fp16_largest(m, *reinterpret_cast<const uint4 *>(smem + (which ? L::Q : L::K) + p * 16));
+                    m = __reduce_max_sync(0xffffffffu, fp16_larger(m));
+                    if (lane == 0) ctl.largest[it & 1][which][warp] = (uint16_t)m;
+                }
+                mbar_arrive(&ctl.meet);
+                ok = mbar_wait_warp(&ctl.meet, it & 1, a.wait_polls);
+                if (!ok) break;
+            }
             // an operand times `weight` of its token, in parts
             const auto parts = [&](int tile, auto weight) {
+                const float f = up(tile == L::Q);
 #pragma unroll 2
                 for (int p = tid; p < KB * TC * 8; p += ARITH) {
                     const int t = (p >> 3) & (TC - 1);
                     uint4 x = *reinterpret_cast<const uint4 *>(smem + tile + p * 16);
                     if (t >= tokens) x = make_uint4(0, 0, 0, 0);
-                    write_parts<T, PARTS>(x, weight(t), smem + L::SPARE + p * 16, KB * BLOCK_BYTES);
+                    write_parts<T, PARTS>(x, HALF ? weight(t) * f : weight(t), smem + L::SPARE + p * 16, KB * BLOCK_BYTES);
                 }
                 fence_async_smem();
                 mbar_arrive(&ctl.ready);
@@ -288,8 +311,9 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             }
             tc_fence_after();
             const f32x2 carry = splat2(exp2f(g2 * (float)e)), steps = splat2((float)e), whole = splat2(1.0f / PART);
-            const f32x2 beyond = splat2(exp2f(g2 * (float)(grows ? e : e - last)));
-            const f32x2 back = splat2(grows ? exp2f(g2 * (float)last) : 1.0f);  // of X and X'
+            const float step = exp2f(g2 * (float)(grows ? e : e - last));
+            const f32x2 beyond = splat2(HALF ? step / up(0) : step);
+            const f32x2 back = splat2(HALF && !STATE_ONLY ? (grows ? exp2f(g2 * (float)last) : 1.0f) / up(1) : 1.0f);  // of X and X'
 #pragma unroll
             for (int c = 0; c < NZ; c += 8) {
                 uint32_t x[8], x1[8], u[8], u1[8];

@@ -14,7 +14,8 @@
 // short sequences 1.4 - 1.6 times as wrong as their rounding).  Z itself and U stay in fp32 and are fp32 results: K~ goes in two
 // parts in fp16 (2^-22) and three in bf16 (2^-25; two, 2^-17, in the passes of a gradient that return no state).  The tensor cores cut the last bits of a sum off at every step of 16 tokens,
 // so small parts are added up first: final states are within 1.5e-7 (2-norm, as an fp32 evaluation is) instead of 5e-7, and
-// 2.4e-6 with two parts of bf16.  fp16 has too few exponents for P and Z: both are scaled by powers of two per row, taken back in
+// 2.4e-6 with two parts of bf16.  fp16 has too few exponents for P, Z and K~: they are scaled by powers of two, P and Z per row, K~ per
+// chunk (its low part is then good to 2^-39 of the chunk's largest key; unscaled, to 2^-25: keys of 1e-3 made states 3e-5 wrong), taken back in
 // fp32.
 //
 // What bounds it: a chunk of a head with dk = dv = 128 moves 128 KB, 5600 cycles of its SM's share of HBM, but 670 KB through
@@ -55,18 +56,12 @@ struct Control {
     __nv_bfloat16 p_scale[2][TC];   // fp16: power of two that takes the scaling of P's row back, by parity of the chunk
     __nv_bfloat16 z_scale[2][128];  // fp16: power of two that takes the scaling of Z's row back, by parity of the chunk
     uint8_t row_max[2][2][TC];      // fp16: exponent of a row's largest magnitude in each half, for either group
+    uint16_t key_max[2][GROUP / 32];  // fp16: largest magnitude of the keys that a warp has seen, as its bits, by parity of the chunk
+    float key_scale[2];             // fp16: power of two that takes the scaling of K~ back
 };
 
 // tensor memory columns
 constexpr uint32_t COL_S = 0, COL_PV = 128, COL_QZ = 256, COL_U = 384;
-
-__device__ __forceinline__ int exponent_of(float m) { return (int)((__float_as_uint(m) >> 23) & 0xffu); }
-// 2^n that brings a largest magnitude of (biased) exponent e to [2^13, 2^14) (fp16's range and as many of its small values as
-// possible); 1 for 0 and for what is not finite
-__device__ __forceinline__ float fp16_scale(int e) {
-    if (e == 0 || e == 255) return 1.0f;
-    return __uint_as_float((uint32_t)min(max(127 + 13 - (e - 127), 2), 252) << 23);  // (its inverse is a normal number too)
-}
 
 // The swizzle of rows of PITCH bytes, 128 or 64, on an offset from a boundary of 1024 bytes.
 template <int PITCH>
@@ -282,6 +277,19 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 for (int p = mine; p < VB * TC * 8; p += GROUP)
                     if (((p >> 3) & (TC - 1)) >= tokens) *reinterpret_cast<uint4 *>(vt + p * 16) = make_uint4(0, 0, 0, 0);
             }
+            float key_up = 1.0f;
+            // K~ is scaled by the chunk's largest key: values below fp16's normal range would leave their low parts no bits
+            if (HALF) {
+                const unsigned char *kt = smem + b * L::STAGE + L::K + mine * 16;
+                uint32_t largest = 0;
+#pragma unroll
+                for (int i = 0; i < KB * 4; i++) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(kt + i * (GROUP * 16));
+                    if ((mine >> 3) + 32 * (i & 3) < tokens) largest = fp16_largest(largest, x);
+                }
+                const uint32_t top = __reduce_max_sync(0xffffffffu, fp16_larger(largest));
+                if (lane == 0) ctl.key_max[it & 1][warp & 7] = (uint16_t)top;
+            }
             if (!STATE_ONLY) {
                 ok = mbar_wait_warp(&ctl.s_full, it & 1, a.wait_polls);
                 if (!ok) break;
@@ -353,6 +361,15 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 tmem_st_wait();
                 tc_fence_before();
             }
+            if (HALF) {
+                if (STATE_ONLY) ok = meet();  // (else they have met for the rows of S)
+                if (!ok) break;
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < GROUP / 32; i++) top = max(top, (uint32_t)ctl.key_max[it & 1][i]);
+                key_up = fp16_scale_of_bits(top);
+                if (mine == 0) ctl.key_scale[it & 1] = 1.0f / key_up;
+            }
             // K~ over K, its low part over Q and, if there is one, its lowest over Z, which QZ has read by now
             const bool three = !HALF && a.parts == 3;
             if (!STATE_ONLY)
@@ -368,7 +385,8 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 // (rows behind the last token are zero, whatever is in them)
                 if (m >= tokens) x = make_uint4(0, 0, 0, 0);
                 // decay to the chunk's last token; where it grows in fp16, relative to that of the chunk's first
-                const f32x2 w = splat2(exp2f(g2 * (float)(max(a.reverse ? m : tokens - 1 - m, 0) - (grows ? tokens - 1 : 0))));
+                const float decay = exp2f(g2 * (float)(max(a.reverse ? m : tokens - 1 - m, 0) - (grows ? tokens - 1 : 0)));
+                const f32x2 w = splat2(HALF ? decay * key_up : decay);
                 const uint32_t in[4] = {x.x, x.y, x.z, x.w};
                 uint32_t high[4], low[4], lowest[4];
 #pragma unroll
@@ -393,6 +411,9 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                 *reinterpret_cast<uint4 *>(qt + i * (GROUP * 16)) = make_uint4(low[0], low[1], low[2], low[3]);
             }
             fence_async_smem();
+            // (states alone: no further ahead than one chunk, of which key_scale has two)
+            if (HALF && STATE_ONLY && it > 0) ok = mbar_wait_warp(&ctl.z_ready, (it - 1) & 1, a.wait_polls);
+            if (!ok) break;
             mbar_arrive(&ctl.p_ready);
         }
         if (!ok) ctl.dead = 1;
@@ -473,14 +494,15 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
             const float carry = exp2f(g2 * (float)e);
             if (it == 0 || tokens < TC) inter = exp2f(g2 * (float)(a.reverse ? tokens - 1 - row : row)) * a.scale_out;
             ok = mbar_wait_warp(&ctl.o_full, it & 1, a.wait_polls);
-            if (HALF && !STATE_ONLY) ok = ok && mbar_wait_warp(&ctl.p_ready, it & 1, a.wait_polls);  // (p_scale; long complete)
+            if (HALF) ok = ok && mbar_wait_warp(&ctl.p_ready, it & 1, a.wait_polls);  // (p_scale, key_scale; long complete)
             ok = ok && *reinterpret_cast<volatile int *>(&ctl.dead) == 0;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             // (K~ is decayed to the chunk's last token, which keeps its largest entries in fp16's range; the step beyond it, and those that growing
             // keys are short of, are taken here)
-            const f32x2 carry2 = splat2(carry), in2 = splat2(a.scale_in * exp2f(g2 * (float)(grows ? e : e - tokens + 1)));
+            const float beyond = a.scale_in * exp2f(g2 * (float)(grows ? e : e - tokens + 1));
+            const f32x2 carry2 = splat2(carry), in2 = splat2(HALF ? beyond * ctl.key_scale[it & 1] : beyond);
 #pragma unroll
             for (int cb = 0; cb < NZ / 16; cb++) {
                 uint32_t r[16];

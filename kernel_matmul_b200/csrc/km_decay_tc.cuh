@@ -88,6 +88,23 @@ __device__ __forceinline__ void two_parts(float a, float b, uint32_t &high, uint
     low = pack<T>(a - h.x, b - h.y);
 }
 
+__device__ __forceinline__ int exponent_of(float m) { return (int)((__float_as_uint(m) >> 23) & 0xffu); }
+// 2^n that brings a largest magnitude of (biased) exponent e to [2^13, 2^14) (fp16's range and as many of its small values as
+// possible); 1 for 0 and for what is not finite
+__device__ __forceinline__ float fp16_scale(int e) {
+    if (e == 0 || e == 255) return 1.0f;
+    return __uint_as_float((uint32_t)min(max(127 + 13 - (e - 127), 2), 252) << 23);  // (its inverse is a normal number too)
+}
+// The larger magnitudes of pairs of fp16 values, as bits; those of a word's two as one.
+__device__ __forceinline__ uint32_t fp16_largest(uint32_t so_far, const uint4 &x) {
+    const uint32_t p = __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), q = __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu);
+    return __vmaxu2(so_far, __vmaxu2(p, q));
+}
+__device__ __forceinline__ uint32_t fp16_larger(uint32_t pair) { return max(pair >> 16, pair & 0xffffu); }
+__device__ __forceinline__ float fp16_scale_of_bits(uint32_t bits) {
+    return fp16_scale(exponent_of(__half2float(__ushort_as_half((unsigned short)bits))));
+}
+
 // Whether every row starts on a boundary of 16 bytes.
 __device__ __forceinline__ bool rows_aligned(const Operand &o, int size) {
     return o.col == 1 && ((reinterpret_cast<uintptr_t>(o.data) | (uintptr_t)((o.seq | o.group | o.head | o.row) * size)) & 15) == 0;
