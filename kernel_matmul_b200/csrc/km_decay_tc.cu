@@ -306,13 +306,14 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                     for (int c0 = half * 16; c0 < TC; c0 += 32) {
                         const int side = a.reverse ? r0 - (c0 & ~31) : (c0 & ~31) - r0, d = row - c0, live = a.reverse ? tokens - c0 : 16;
                         if (side > 0 || live <= 0) continue;
+                        const int lo = a.reverse ? d : 0, hi = a.reverse ? live - 1 : d;  // the row's columns of the block
                         uint32_t r[16];
                         tmem_ld16_nowait(lanes + COL_S + c0, r);
                         tmem_ld_wait16(r);
                         float largest = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 16; j++)
-                            largest = fmaxf(largest, (side < 0 || (a.reverse ? j >= d : j <= d)) && j < live ? fabsf(__uint_as_float(r[j])) : 0.0f);
+                            largest = fmaxf(largest, j >= lo && j <= hi ? fabsf(__uint_as_float(r[j])) : 0.0f);
                         if (grows) largest *= ex2_approx(g2 * (float)max(a.reverse ? 15 - d : d, 0));  // (its farthest column)
                         m = fmaxf(m, largest);
                     }
@@ -344,6 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                                 two_parts<T>(u, v, w[j], w[j + 8]);
                             }
                         } else {  // entry by entry
+                            const int lo = a.reverse ? d : 0, hi = a.reverse ? live - 1 : d;
                             const f32x2 g22 = splat2(a.reverse ? -g2 : g2), d2 = splat2((float)d), up2 = splat2(up);
                             tmem_ld_wait16(r);
 #pragma unroll
@@ -351,8 +353,7 @@ __global__ void __launch_bounds__(THREADS, 1) decay_tc_kernel(const __grid_const
                                 const f32x2 x = ex2_approx2(mul2(g22, sub2(d2, pack2((float)(2 * j), (float)(2 * j + 1)))));
                                 float u, v;
                                 unpack2(mul2(HALF ? mul2(x, up2) : x, pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]))), u, v);
-                                two_parts<T>((a.reverse ? 2 * j >= d : 2 * j <= d) && 2 * j < live ? u : 0.0f,
-                                             (a.reverse ? 2 * j + 1 >= d : 2 * j + 1 <= d) && 2 * j + 1 < live ? v : 0.0f, w[j], w[j + 8]);
+                                two_parts<T>(2 * j >= lo && 2 * j <= hi ? u : 0.0f, 2 * j + 1 >= lo && 2 * j + 1 <= hi ? v : 0.0f, w[j], w[j + 8]);
                             }
                         }
                     }
