@@ -230,10 +230,9 @@ template <bool TANGENT>
 __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
     const unsigned h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
     const unsigned hg = h / a.group, hi = h - hg * a.group;
-    const int slot0 = segments_before(a, seq);
     int64_t begin, length;
     sequence_rows(a, seq, begin, length);
-    const int place = slot0 - (int)seq;
+    const int64_t place = first_place(a, seq);
     const int n = (int)min((int64_t)segments_of(a, length) - 1, a.state_slots - place);
     if (n <= 0) return;
     const float g2 = log2_decay(a.log_decay[h]);
@@ -248,7 +247,7 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(DecayArgs a) {
                           ? enter * a.state_in.at<float>(seq, hg, hi)[(i / a.dv) * a.state_in.row + (i % a.dv) * a.state_in.col]
                           : 0.0f;
     }
-    float *p = a.states + ((int64_t)place * a.heads + h) * N * values + first;
+    float *p = a.states + (place * a.heads + h) * N * values + first;
     const int64_t step = (int64_t)a.heads * N * values;
     const float tokens = (float)a.segment;
     for (int j = 0; j < n; j += 4) {

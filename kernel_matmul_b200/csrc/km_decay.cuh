@@ -100,74 +100,64 @@ __device__ __forceinline__ int segments_of(const DecayArgs &a, int64_t length) {
     return length <= a.segment ? 1 : (int)(((unsigned)length + (a.segment - 1u)) / a.segment);
 }
 
-// Segments of the sequences before `seq` (all lanes of a warp call it, all get the result).
-__device__ __forceinline__ int segments_before(const DecayArgs &a, int64_t seq) {
-    if (a.starts == nullptr) return (int)seq * segments_of(a, a.tokens);
-    int sum = 0;
-    for (int64_t i = threadIdx.x & 31; i < seq; i += 32) {
-        int64_t begin, length;
-        sequence_rows(a, i, begin, length);
-        sum += segments_of(a, length);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+// Packed sequences: sequence i, which starts at row b, has its segments in the slots from i + floor(b / segment) on and its states in the
+// places from floor(b / segment) on.  A sequence of n rows has at most floor((b + n) / segment) - floor(b / segment) + 1 segments and
+// one state less, so the next one's come behind, and neither needs a sum over the sequences before.  (No `starts` leads out of the slots and
+// places there are; those that decrease may give two sequences the same ones.)
+__device__ __forceinline__ int64_t first_place(const DecayArgs &a, int64_t i) {
+    if (a.starts == nullptr) return i * (segments_of(a, a.tokens) - 1);
+    return (unsigned)min(max((int64_t)a.starts[i], (int64_t)0), a.tokens) / a.segment;
 }
 
 // Segment number `slot` (one warp calls it, all lanes get the result).
 __device__ __forceinline__ Segment find_segment(const DecayArgs &a, int64_t slot) {
     Segment r = {};
     r.spare = -1;
-    int index = 0;
+    int64_t index = 0, place = 0;
     if (a.starts == nullptr) {
         const int per = segments_of(a, a.tokens);
         r.seq = (int)((unsigned)slot / (unsigned)per);
         index = (int)slot - r.seq * per;
-        r.used = true;
+        place = (int64_t)r.seq * (per - 1);
     } else {
-        const int lane = threadIdx.x & 31;
-        int before = 0;
-        for (int64_t base = 0; base < a.sequences && !r.used; base += 32) {
-            const int64_t i = base + lane;
-            int64_t begin, length = 0;
-            int n = 0;
-            if (i < a.sequences) {
-                sequence_rows(a, i, begin, length);
-                n = segments_of(a, length);
-            }
-            int upto = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
-            }
-            upto += before;
-            const unsigned hit = __ballot_sync(0xffffffffu, slot < upto);
-            if (hit != 0) {
-                const int who = __ffs(hit) - 1;
-                r.seq = (int)base + who;
-                index = (int)slot - __shfl_sync(0xffffffffu, upto - n, who);
-                r.used = true;
-            }
-            before = __shfl_sync(0xffffffffu, upto, 31);
+        // rows of no sequence: for the slots before the first sequence's and behind the last one's, or, if there are none, the last slot
+        const int64_t begin = first_place(a, 0), end = a.sequences + first_place(a, a.sequences);
+        int64_t spares = begin + (a.slots - end);
+        if (slot < begin)
+            r.spare = (int)slot;
+        else if (slot >= end)
+            r.spare = (int)(begin + (slot - end));
+        else if (spares == 0 && slot == a.slots - 1)
+            r.spare = 0, spares = 1;
+        r.spares = (int)spares;
+        // the last sequence whose first slot is not behind this one: 32 candidates at a time
+        int64_t first = 0, count = a.sequences;
+        bool found = false;
+        for (int64_t step = count; step > 0 && !(found && step == 1);) {
+            step = (count + 31) / 32;
+            const int64_t i = first + (threadIdx.x & 31) * step;
+            const unsigned hit = __ballot_sync(0xffffffffu, i < first + count && i + first_place(a, i) <= slot);
+            if (hit == 0) break;
+            const int64_t skip = (31 - __clz(hit)) * step;
+            first += skip, count = min(step, count - skip);
+            found = true;
         }
-        if (!r.used) {
-            r.spare = (int)(slot - before);
-            r.spares = (int)(a.slots - before);
-            return r;
-        }
+        if (!found) return r;
+        r.seq = (int)first;
+        place = first_place(a, first);
+        index = slot - (first + place);
     }
     int64_t begin, length;
     sequence_rows(a, r.seq, begin, length);
+    const int segments = segments_of(a, length);
+    if (index >= segments) return r;  // (of packed sequences some slots are left over)
+    r.used = true;
     r.begin = (int)begin, r.length = (int)length;
-    r.first = index * (int)a.segment;
-    r.last = index == segments_of(a, length) - 1;
-    // (a sequence of n segments has n - 1 states; bounded, should `starts` decrease and sequences overlap)
-    r.adds = (int)min(slot - r.seq, a.state_slots - 1);
-    r.start = (int)min(slot - r.seq - 1, a.state_slots - 1);
+    r.first = (int)index * (int)a.segment;
+    r.last = index == segments - 1;
+    r.adds = (int)min(place + index, a.state_slots - 1);
+    r.start = (int)min(place + index - 1, a.state_slots - 1);
     r.count = min(r.length - r.first, (int)a.segment);
-    // the very last slot is in use: its CTA sees to the rows of no sequence
-    if (a.starts != nullptr && slot == a.slots - 1) r.spare = 0, r.spares = 1;
     return r;
 }
 
