@@ -568,7 +568,7 @@ KM_API int km_node_product_f32(int64_t k, int64_t n, int64_t nodes_per_block, in
  * generated on the fly, here over the tokens of sequences.
  *
  * Element types (`KM_TYPE_*`) are given per call; state, decays, norms and gradients of decays are fp32.
- * Strides are in elements, int64.
+ * Strides are in elements, int64.  Workspaces: 16-byte aligned, contents irrelevant on entry unless said otherwise.
  * ------------------------------------------------------------------------------------- */
 #define KM_TYPE_F32 0
 #define KM_TYPE_BF16 1

@@ -732,6 +732,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     const size_t need = km_decay_attention_workspace_bytes(problem);
     KM_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KM_ERR_WORKSPACE,
                "km_decay_attention: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    KM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_decay_attention: workspace must be 16-byte aligned");
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.out = make_operand(out);
     a.state_out = make_operand(state_out);
@@ -811,9 +812,12 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
     if (rc != KM_OK) return rc;
     if (p.groups == 0) return KM_OK;
     KM_REQUIRE(q && k && v && dout && log_decay && grad && (!p.packed || starts), KM_ERR_INVALID_ARGUMENT, "km_decay_gradient: null argument");
+    KM_REQUIRE(p.tokens == 0 || p.sequences == 0 || (q->data && k->data && v->data && dout->data), KM_ERR_INVALID_ARGUMENT,
+               "km_decay_gradient: null pointer");
     const size_t need = km_decay_gradient_workspace_bytes(problem);
     KM_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KM_ERR_WORKSPACE,
                "km_decay_gradient: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    KM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_decay_gradient: workspace must be 16-byte aligned");
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.scale_in = 1.0f, a.scale_out = p.scale;
     const Operand d = make_operand(dout), ds = make_operand(dstate);
@@ -846,8 +850,11 @@ extern "C" int km_group_sums(int32_t dtype, int64_t rows, int64_t groups, int64_
     using namespace km;
     KM_REQUIRE(dtype >= KM_TYPE_F32 && dtype <= KM_TYPE_F16 && rows >= 0 && groups >= 0 && group >= 1 && dim >= 0, KM_ERR_INVALID_ARGUMENT,
                "km_group_sums: bad arguments");
+    if (rows == 0 || groups == 0 || dim == 0) return KM_OK;
+    const int64_t limit = 1LL << 60;  // values of `in`
+    KM_REQUIRE(groups <= limit / rows && dim <= limit / (rows * groups) && group <= limit / (rows * groups * dim), KM_ERR_UNSUPPORTED,
+               "km_group_sums: more than 2^60 values");
     const int64_t count = rows * groups * dim;
-    if (count == 0) return KM_OK;
     KM_REQUIRE(in && out, KM_ERR_INVALID_ARGUMENT, "km_group_sums: null pointer");
     const unsigned ctas = (unsigned)std::min<int64_t>(ceil_div(count, 256), 8LL * sm_count());
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -892,11 +899,13 @@ extern "C" int km_decay_step(int32_t dtype, int64_t rows, int64_t pool, int64_t 
                "km_decay_step: head sizes must be 1 to %d", KM_DECAY_MAX_DIM);
     KM_REQUIRE(slots == nullptr ? rows <= pool : (slot_type == KM_TYPE_I32 || slot_type == KM_TYPE_I64), KM_ERR_INVALID_ARGUMENT,
                "km_decay_step: bad slots");
-    KM_REQUIRE(rows < (1LL << 31) && groups < (1LL << 31) && group < (1LL << 31) && groups * group < (1LL << 31), KM_ERR_UNSUPPORTED,
-               "km_decay_step: more than 2^31 rows or heads");
+    KM_REQUIRE(rows < (1LL << 31) && groups < (1LL << 31) && group < (1LL << 31) && groups * group < (1LL << 31) &&
+                   rows * (groups * group) < (1LL << 31),
+               KM_ERR_UNSUPPORTED, "km_decay_step: more than 2^31 (row, head) pairs");
     if (rows == 0 || groups == 0) return KM_OK;
     KM_REQUIRE(q && k && v && out && log_decay && states && q->data && k->data && v->data && out->data, KM_ERR_INVALID_ARGUMENT,
                "km_decay_step: null argument");
+    KM_REQUIRE(pool == 0 || states->data, KM_ERR_INVALID_ARGUMENT, "km_decay_step: null pointer");
     KM_REQUIRE(q->stride[1] == 1 && k->stride[1] == 1 && v->stride[1] == 1 && out->stride[1] == 1 && states->stride[1] == 1,
                KM_ERR_INVALID_ARGUMENT, "km_decay_step: values of a head must be contiguous");
     const Operand oq = make_operand(q), ok = make_operand(k), ov = make_operand(v), oo = make_operand(out), os = make_operand(states);

@@ -265,6 +265,7 @@ extern "C" int km_global_norm(int64_t count, void *const *tensors, const int64_t
                "km_global_norm: bad arguments");
     KM_REQUIRE(workspace != nullptr && workspace_bytes >= km_global_norm_workspace_bytes(count), KM_ERR_WORKSPACE,
                "km_global_norm: workspace of %zu bytes needed", km_global_norm_workspace_bytes(count));
+    KM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_global_norm: workspace must be 16-byte aligned");
     for (int64_t i = 0; i < count; i++) {
         KM_REQUIRE(elements[i] >= 0 && types[i] >= KM_TYPE_F32 && types[i] <= KM_TYPE_F16 && (elements[i] == 0 || tensors[i] != nullptr),
                    KM_ERR_INVALID_ARGUMENT, "km_global_norm: bad tensor %lld", (long long)i);
