@@ -610,9 +610,9 @@ typedef struct km_decay_problem {
     int32_t reverse, path;
     int64_t sequences, tokens, groups, group, dk, dv;
     int32_t packed;
-    /* What the workspace holds.  0: nothing.  1: the states between segments that an earlier call with the same log_decay, k, v,
-     * state_in, starts and sizes left there (q may differ).  2: those of a call with k and v, dk and dv, and the state's dims
-     * swapped: the gradients of k and v run over transposed states, as that of q over those of the forward call. */
+    /* What the workspace holds.  0: nothing.  2: the states between segments that a call with the same log_decay, state_in, starts and sizes, but
+     * k and v, dk and dv, and the state's dims swapped, left there (q may differ): the gradients of k and v run over transposed states, as that of q
+     * over those of the forward call. */
     int32_t states;
     float scale;
 } km_decay_problem;

@@ -646,7 +646,7 @@ static int check_problem(const char *name, const km_decay_problem *p) {
     KM_REQUIRE(p->path == 1 || (p->path == 2 && p->dtype != KM_TYPE_F32), KM_ERR_UNSUPPORTED,
                "%s: path must be 1 (FMA pipe) or, for 16-bit types, 2 (tensor cores)", name);
     KM_REQUIRE(p->reverse >= 0 && p->reverse <= 2, KM_ERR_INVALID_ARGUMENT, "%s: reverse must be 0, 1 or 2", name);
-    KM_REQUIRE(p->states >= 0 && p->states <= 2, KM_ERR_INVALID_ARGUMENT, "%s: states must be 0, 1 or 2", name);
+    KM_REQUIRE(p->states == 0 || p->states == 2, KM_ERR_INVALID_ARGUMENT, "%s: states must be 0 or 2", name);
     KM_REQUIRE(p->sequences >= 0 && p->tokens >= 0 && p->groups >= 0 && p->group >= 1, KM_ERR_INVALID_ARGUMENT, "%s: bad sizes", name);
     KM_REQUIRE(p->dk >= 1 && p->dk <= KM_DECAY_MAX_DIM && p->dv >= 1 && p->dv <= KM_DECAY_MAX_DIM, KM_ERR_UNSUPPORTED,
                "%s: head sizes must be 1 to %d", name, KM_DECAY_MAX_DIM);

@@ -62,3 +62,10 @@ def test_workspaces_off_their_boundary():
     refused(lib.km_decay_gradient(p, v, v, v, v, ANY, None, None, None, ANY, off, lib.km_decay_gradient_workspace_bytes(p), None), b"16-byte aligned")
     one = (ctypes.c_void_p * 1)(4096), (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(0)
     refused(lib.km_global_norm(1, *one, 0, 0.0, 0.0, ANY, off, lib.km_global_norm_workspace_bytes(1), None), b"16-byte aligned")
+
+
+@pytest.mark.parametrize("states", [1, -1, 3])
+def test_workspaces_that_hold_something_else(states):
+    p = KmDecayProblem(dtype=0, out_dtype=0, reverse=0, path=0, sequences=1, tokens=8, groups=2, group=1, dk=16, dv=16, packed=0, states=states, scale=1.0)
+    v = view()
+    refused(lib.km_decay_attention(p, v, v, v, v, ANY, None, None, None, ANY, 0, None), b"states must be")
