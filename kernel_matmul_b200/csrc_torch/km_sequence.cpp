@@ -1,8 +1,10 @@
 // The sequence operators: argument checks, views, allocation and autograd for km_rotary, km_decay_attention,
 // km_decay_gradient, km_decay_step and km_global_norm.
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
@@ -38,6 +40,14 @@ static bool recording(std::initializer_list<const Tensor *> inputs) {
     for (const Tensor *t : inputs)
         if (t->defined() && ((t->requires_grad() && at::GradMode::is_enabled()) || t->_fw_grad(0).defined())) return true;
     return false;
+}
+
+// torch.jit.trace and make_fx see the allocation of a result and not the kernel that fills it: what they recorded would return
+// memory as it comes.
+static void refuse_recordings(const char *name) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                name, " cannot be recorded by torch.jit.trace or make_fx");
 }
 
 // In-place writes past autograd's back are counted, so that a graph that saved the tensor notices.
@@ -126,6 +136,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 
 std::vector<Tensor> rotary(const Tensor &q, const Maybe &k, const Tensor &positions, const Tensor &frequencies, bool interleaved,
                            double scale) {
+    refuse_recordings("rotary");
     std::vector<Tensor> xs{q};
     if (k.has_value()) xs.push_back(*k);
     type_of(q, "q");
@@ -312,6 +323,7 @@ static double scale_for(std::optional<double> scale, int64_t dk) { return scale.
 
 std::vector<Tensor> decay_attention(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, std::optional<double> scale,
                                     const Maybe &initial_state, const Maybe &starts, bool return_state, int64_t path) {
+    refuse_recordings("decay_attention");
     DecayCall c{};
     c.type = type_of(q, "q");
     type_of(k, "k"), type_of(v, "v"), check_f32(log_decay);
@@ -375,6 +387,7 @@ std::vector<Tensor> decay_attention(const Tensor &q, const Tensor &k, const Tens
 
 Tensor decay_attention_step(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, const Tensor &states,
                             std::optional<double> scale, const Maybe &slots) {
+    refuse_recordings("decay_attention_step");
     const int32_t type = type_of(q, "q");
     type_of(k, "k"), type_of(v, "v"), check_f32(log_decay), check_f32(states);
     check_same_device(q, k), check_same_device(q, v), check_same_device(q, log_decay), check_same_device(q, states);
@@ -435,6 +448,7 @@ Tensor decay_attention_step(const Tensor &q, const Tensor &k, const Tensor &v, c
 // ------------------------------------------------------------------------------------------ norm over many tensors
 
 Tensor global_norm(const std::vector<Tensor> &tensors, std::optional<double> max_norm, double eps) {
+    refuse_recordings("global_norm");
     if (tensors.empty()) throw ArgumentError("no tensors given");
     if (max_norm.has_value() && !(*max_norm >= 0.0)) throw ArgumentError("max_norm must not be negative or NaN");
     if (!(eps >= 0.0) || std::isinf(eps)) throw ArgumentError("eps must be finite and not negative");

@@ -350,6 +350,8 @@ def count_entries(m: int, n: int, start: Tensor, end: Tensor) -> Tensor:
 
 # --------------------------------------------------------------------------- sequence operators
 
+# (torch.jit.trace and make_fx cannot record them: such calls are refused.)
+
 
 def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
                        original_tokens: int | None = None, fast_turns: float = 32.0, slow_turns: float = 1.0,
