@@ -3,6 +3,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/VariableTypeUtils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -447,11 +448,7 @@ Tensor decay_attention_step(const Tensor &q, const Tensor &k, const Tensor &v, c
 
 // ------------------------------------------------------------------------------------------ norm over many tensors
 
-Tensor global_norm(const std::vector<Tensor> &tensors, std::optional<double> max_norm, double eps) {
-    refuse_recordings("global_norm");
-    if (tensors.empty()) throw ArgumentError("no tensors given");
-    if (max_norm.has_value() && !(*max_norm >= 0.0)) throw ArgumentError("max_norm must not be negative or NaN");
-    if (!(eps >= 0.0) || std::isinf(eps)) throw ArgumentError("eps must be finite and not negative");
+static Tensor norm_raw(const std::vector<Tensor> &tensors, std::optional<double> max_norm, double eps) {
     const bool scale = max_norm.has_value();
     const size_t n = tensors.size();
     std::vector<Tensor> flat;  // dense storage to work on
@@ -514,6 +511,26 @@ Tensor global_norm(const std::vector<Tensor> &tensors, std::optional<double> max
         }
     }
     return norm;
+}
+
+// A norm of tensors that require a gradient says that it has none where one is asked for, instead of leaving it out of a sum.
+struct NormFunction : torch::autograd::Function<NormFunction> {
+    static Tensor forward(AutogradContext *, at::TensorList tensors) { return norm_raw(tensors.vec(), {}, 0.0); }
+    static variable_list backward(AutogradContext *, variable_list) { TORCH_CHECK(false, "global_norm has no gradient"); }
+};
+
+Tensor global_norm(const std::vector<Tensor> &tensors, std::optional<double> max_norm, double eps) {
+    refuse_recordings("global_norm");
+    if (tensors.empty()) throw ArgumentError("no tensors given");
+    if (max_norm.has_value() && !(*max_norm >= 0.0)) throw ArgumentError("max_norm must not be negative or NaN");
+    if (!(eps >= 0.0) || std::isinf(eps)) throw ArgumentError("eps must be finite and not negative");
+    if (!max_norm.has_value()) {
+        for (const Tensor &t : tensors)
+            if (recording({&t})) return NormFunction::apply(at::TensorList(tensors));
+    } else if (torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr) {  // (the question of each tensor takes a lock)
+        for (const Tensor &t : tensors) TORCH_CHECK(!t._fw_grad(0).defined(), "clip_global_norm_ has no forward-mode derivative");
+    }
+    return norm_raw(tensors, max_norm, eps);
 }
 
 }  // namespace kmh

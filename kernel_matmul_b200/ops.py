@@ -445,7 +445,8 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
 
 def global_norm(tensors: Sequence[Tensor]) -> Tensor:
     """2-norm of the elements of all ``tensors`` (fp32, bf16, fp16, on one CUDA device) as a 0-dim fp32 tensor; one pass, no
-    synchronisation, the same bits for the same tensors.  A tensor that is listed twice counts once."""
+    synchronisation, the same bits for the same tensors.  A tensor that is listed twice counts once.  It has no gradient: a backward
+    pass through the norm of tensors that require one raises."""
     return _C.global_norm(list(tensors), None, 0.0)
 
 

@@ -39,7 +39,7 @@ def test_recordings_without_the_kernels_are_refused(name):
     f(x)  # (and nothing of that stays)
 
 
-@pytest.mark.parametrize("name", ["rotary", "attention", "step"])
+@pytest.mark.parametrize("name", ["rotary", "attention", "step", "norm", "clip"])
 def test_forward_mode_and_transforms_are_refused(name):
     f, x = calls()[name]
     with torch.autograd.forward_ad.dual_level():
@@ -66,3 +66,14 @@ def test_saved_tensors_may_be_moved_away():
     with torch.autograd.graph.save_on_cpu():
         got = step()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_gradient_of_a_norm_is_refused_and_not_left_out():
+    x, y = torch.randn(10, device=DEV).requires_grad_(), torch.randn(3, device=DEV)
+    norm = ops.global_norm([x, y])
+    assert abs(norm.item() - torch.cat([x, y]).norm().item()) < 1e-5
+    with pytest.raises(RuntimeError, match="no gradient"):
+        (x.sum() + norm).backward()
+    with torch.no_grad():
+        assert not ops.global_norm([x]).requires_grad
+    assert not ops.global_norm([x.detach(), y]).requires_grad
