@@ -46,6 +46,9 @@ static bool recording(std::initializer_list<const Tensor *> inputs) {
 // torch.jit.trace and make_fx see the allocation of a result and not the kernel that fills it: what they recorded would return
 // memory as it comes.
 static void refuse_recordings(const char *name) {
+    // (both include keys in this thread's set; asking them costs a quarter of a microsecond)
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::Tracer, c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot});
+    if (!c10::impl::tls_local_dispatch_key_set().included_.has_any(keys)) return;
     TORCH_CHECK(!torch::jit::tracer::isTracing() &&
                     !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
                 name, " cannot be recorded by torch.jit.trace or make_fx");
