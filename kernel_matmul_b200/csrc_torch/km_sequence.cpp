@@ -468,27 +468,27 @@ static Tensor norm_raw(const std::vector<Tensor> &tensors, std::optional<double>
     }
     const c10::cuda::CUDAGuard guard(tensors[0].device());
     // a tensor that is listed twice counts once and is scaled once; tensors that overlap otherwise are not scaled at all
+    std::vector<uintptr_t> begin(n), end(n, 0);
+    for (size_t i = 0; i < n; i++) begin[i] = reinterpret_cast<uintptr_t>(tensors[i].data_ptr());
     std::vector<size_t> order(n);
     std::iota(order.begin(), order.end(), (size_t)0);
-    const auto begin = [&](size_t i) { return reinterpret_cast<uintptr_t>(tensors[i].data_ptr()); };
-    std::stable_sort(order.begin(), order.end(), [&](size_t a, size_t b) { return begin(a) < begin(b); });
+    std::stable_sort(order.begin(), order.end(), [&](size_t a, size_t b) { return begin[a] < begin[b]; });
     std::vector<char> repeated(n, 0);
-    uintptr_t upto = 0;
-    size_t last = n;
+    std::vector<size_t> open;  // earlier tensors that reach behind this one's first element
     for (size_t i : order) {
-        if (tensors[i].numel() == 0) continue;
+        const Tensor &t = tensors[i];
+        if (t.numel() == 0) continue;
         // (the extent of a view with gaps)
         uintptr_t span = 1;
-        for (int64_t d = 0; d < tensors[i].dim(); d++) span += (uintptr_t)((tensors[i].size(d) - 1) * tensors[i].stride(d));
-        const uintptr_t end = begin(i) + span * tensors[i].itemsize();
-        if (last < n && begin(i) == begin(last) && tensors[i].sizes() == tensors[last].sizes() && tensors[i].strides() == tensors[last].strides() &&
-            tensors[i].scalar_type() == tensors[last].scalar_type()) {
-            repeated[i] = 1;
-            continue;
-        }
-        TORCH_CHECK(!scale || begin(i) >= upto, "tensors to clip must not overlap");
-        if (end > upto) upto = end;
-        last = i;
+        for (int64_t d = 0; d < t.dim(); d++) span += (uintptr_t)((t.size(d) - 1) * t.stride(d));
+        end[i] = begin[i] + span * t.itemsize();
+        open.erase(std::remove_if(open.begin(), open.end(), [&](size_t j) { return end[j] <= begin[i]; }), open.end());
+        for (size_t j : open)
+            repeated[i] = repeated[i] || (begin[i] == begin[j] && t.sizes() == tensors[j].sizes() && t.strides() == tensors[j].strides() &&
+                                          t.scalar_type() == tensors[j].scalar_type());
+        if (repeated[i]) continue;
+        TORCH_CHECK(!scale || open.empty(), "tensors to clip must not overlap");
+        open.push_back(i);
     }
     std::vector<void *> data;
     std::vector<int64_t> elements;
