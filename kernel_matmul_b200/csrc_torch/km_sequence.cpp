@@ -451,6 +451,54 @@ Tensor decay_attention_step(const Tensor &q, const Tensor &k, const Tensor &v, c
 
 // ------------------------------------------------------------------------------------------ norm over many tensors
 
+// Whether views `a` and `b` are shown to share no element.  With strides S_1 > S_2 > .. > 1 of both, an element at offset
+// i_1 S_1 + i_2 S_2 + .. has these numbers as digits, and only these as long as no digit with all below it reaches the stride above.  A
+// view's elements are a box in the digits; they are apart where the boxes are, in any one digit.
+static bool apart_from(const Tensor &a, const Tensor &b, uintptr_t origin) {
+    const int64_t size = a.itemsize();
+    if (b.itemsize() != size) return false;
+    std::vector<int64_t> strides{1};
+    for (const Tensor *t : {&a, &b})
+        for (int64_t d = 0; d < t->dim(); d++)
+            if (t->size(d) > 1) strides.push_back(t->stride(d));
+    std::sort(strides.begin(), strides.end(), std::greater<>());
+    strides.erase(std::unique(strides.begin(), strides.end()), strides.end());
+    if (strides.back() < 1) return false;
+    const size_t n = strides.size();
+    std::vector<int64_t> first[2], behind[2];
+    for (int which = 0; which < 2; which++) {
+        const Tensor &t = which ? b : a;
+        const uintptr_t from = reinterpret_cast<uintptr_t>(t.data_ptr()) - origin;
+        if (from % size != 0) return false;
+        int64_t rest = (int64_t)(from / size);
+        for (size_t i = 0; i < n; i++) {
+            first[which].push_back(rest / strides[i]), rest %= strides[i];
+            int64_t count = 1;
+            for (int64_t d = 0; d < t.dim(); d++) {
+                if (t.size(d) <= 1 || t.stride(d) != strides[i]) continue;
+                if (count > 1) return false;  // (two dims of one stride)
+                count = t.size(d);
+            }
+            behind[which].push_back(first[which][i] + count);
+        }
+    }
+    bool apart = false;
+    int64_t below = 0;  // the largest offset of the digits below
+    for (size_t i = n; i-- > 0;) {
+        if (below >= strides[i]) return false;
+        if (i > 0) below += (std::max(behind[0][i], behind[1][i]) - 1) * strides[i];
+        apart = apart || behind[0][i] <= first[1][i] || behind[1][i] <= first[0][i];
+    }
+    return apart;
+}
+
+// Seen from the start of their buffer, or from the first of them.
+static bool apart(const Tensor &a, const Tensor &b) {
+    const auto at = [](const Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    const auto buffer = [](const Tensor &t) { return reinterpret_cast<uintptr_t>(t.storage().data()); };
+    return (buffer(a) == buffer(b) && apart_from(a, b, buffer(a))) || apart_from(a, b, std::min(at(a), at(b)));
+}
+
 static Tensor norm_raw(const std::vector<Tensor> &tensors, std::optional<double> max_norm, double eps) {
     const bool scale = max_norm.has_value();
     const size_t n = tensors.size();
@@ -487,7 +535,8 @@ static Tensor norm_raw(const std::vector<Tensor> &tensors, std::optional<double>
             repeated[i] = repeated[i] || (begin[i] == begin[j] && t.sizes() == tensors[j].sizes() && t.strides() == tensors[j].strides() &&
                                           t.scalar_type() == tensors[j].scalar_type());
         if (repeated[i]) continue;
-        TORCH_CHECK(!scale || open.empty(), "tensors to clip must not overlap");
+        if (scale)
+            for (size_t j : open) TORCH_CHECK(apart(tensors[j], t), "tensors to clip must not overlap");
         open.push_back(i);
     }
     std::vector<void *> data;

@@ -453,7 +453,7 @@ def global_norm(tensors: Sequence[Tensor]) -> Tensor:
 def clip_global_norm_(tensors: Sequence[Tensor], max_norm: float, *, eps: float = 1e-6) -> Tensor:
     """``global_norm`` of the gradients ``tensors``, which are multiplied in place by ``min(1, max_norm / (norm + eps))``.  Returns
     the norm before.  Where that factor is one the tensors are not written; a norm that is not finite gives what the formula
-    gives.  Tensors that overlap in part are refused."""
+    gives.  Slices of one buffer that share no element are taken, tensors that overlap (or whose strides leave that open) refused."""
     return _C.global_norm(list(tensors), float(max_norm), float(eps))
 
 

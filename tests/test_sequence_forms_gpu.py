@@ -1,6 +1,8 @@
 """Sequence operators under forms of calls of PyTorch's that would go past their kernels."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -88,3 +90,52 @@ def test_a_tensor_that_is_listed_twice_counts_once():
         want = sum(square(t) for t in once) ** 0.5
         # squares and sums of up to 128 of them in fp32, fp64 beyond: off by 131 half steps, its root by half
         assert abs(ops.global_norm(views).item() - want) <= want * 66 * 2.0**-24
+
+
+# ------------------------------------------------------------------------------------------ views of one buffer
+
+
+def clipped_apart(views, base):
+    """Clipping ``views`` of ``base`` gives what clipping copies of them gives, and leaves the rest of ``base``."""
+    copies = [t.clone() for t in views]
+    outside = base.clone()
+    norm = ops.clip_global_norm_(copies, 0.5)
+    got = ops.clip_global_norm_(views, 0.5)
+    # (the copies lie elsewhere: sums in another order)
+    assert abs(got.item() - norm.item()) <= 1e-5 * norm.item()
+    for a, b in zip(views, copies):
+        assert torch.allclose(a.float(), b.float(), rtol=2 * torch.finfo(a.dtype).eps, atol=0.0)
+    mask = torch.zeros_like(base, dtype=torch.bool)
+    flat = mask.flatten()
+    for t in views:
+        torch.as_strided(flat, t.size(), t.stride(), t.storage_offset() - base.storage_offset()).fill_(True)
+    assert torch.equal(base.flatten()[~flat], outside.flatten()[~flat])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_slices_of_one_buffer_are_clipped(dtype):
+    new = lambda *s: torch.randn(s, device=DEV).to(dtype)  # noqa: E731
+    base = new(20, 36)
+    clipped_apart(list(base.chunk(3, dim=1)), base)
+    base = new(20, 36)
+    clipped_apart([base[:, 24:], base[5:, :12], base[3:17, 12:20]], base)
+    base = new(36, 20).t()
+    clipped_apart([base[2:, :12], base[:2, 3:]], base.t())
+    base = new(4, 6, 5, 8)
+    clipped_apart([base[:, :3, :, 2:6], base[1:, 3:, 1:3], base[:, :3, :, 6:], base[2:, :3, :, :2]], base)
+    base = new(100)
+    clipped_apart([base[::2], base[1::2]], base)
+    base = new(101)
+    clipped_apart([base[::3], base[2::3], base[1:50:3]], base)
+
+
+def test_slices_that_overlap_are_refused():
+    base = torch.randn(20, 36, device=DEV)
+    before = base.clone()
+    line = base.flatten()
+    for views in ([base[:, :13], base[:, 12:]], [base[:10], base[9:]], [base[:, :12], base[3:4]], [base[::2], base[2:3]], [base, base[:, 5:]],
+                  [base, base.t()], [line[::2], line[::3]], [line[:1], line[0:700:5]]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.clip_global_norm_(list(views), 0.5)
+    assert torch.equal(base, before)
+    assert abs(ops.global_norm([base, base[:, 5:]]).item() - math.sqrt(base.square().sum().item() + base[:, 5:].square().sum().item())) < 1e-3
