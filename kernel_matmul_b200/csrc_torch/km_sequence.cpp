@@ -548,10 +548,9 @@ static Tensor norm_raw(const std::vector<Tensor> &tensors, std::optional<double>
     }
     Tensor norm = at::empty({}, tensors[0].options().dtype(at::kFloat).requires_grad(false));
     const Tensor ws = workspace(norm, km_global_norm_workspace_bytes((int64_t)data.size()));
-    const bool bounded = scale && !std::isinf(*max_norm);
-    raise_on(km_global_norm((int64_t)data.size(), data.data(), elements.data(), types.data(), bounded, max_norm.value_or(0.0), eps,
+    raise_on(km_global_norm((int64_t)data.size(), data.data(), elements.data(), types.data(), scale, max_norm.value_or(0.0), eps,
                             norm.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream_of(norm)));
-    if (bounded) {
+    if (scale) {
         for (size_t i = 0; i < n; i++) {
             if (repeated[i]) continue;
             if (flat[i].is_same(tensors[i])) {

@@ -139,3 +139,20 @@ def test_slices_that_overlap_are_refused():
             ops.clip_global_norm_(list(views), 0.5)
     assert torch.equal(base, before)
     assert abs(ops.global_norm([base, base[:, 5:]]).item() - math.sqrt(base.square().sum().item() + base[:, 5:].square().sum().item())) < 1e-3
+
+
+# ------------------------------------------------------------------------------------------ bounds that are not finite
+
+
+def test_an_infinite_bound_gives_what_the_formula_gives():
+    x = torch.randn(10, device=DEV)
+    kept = x.clone()
+    ops.clip_global_norm_([x], math.inf)
+    assert torch.equal(x, kept)
+    x[3] = math.nan
+    assert math.isnan(ops.clip_global_norm_([x], math.inf).item()) and x.isnan().all()  # inf / (nan + eps)
+    y = torch.tensor([math.inf, 1.0], device=DEV)
+    assert math.isinf(ops.clip_global_norm_([y], math.inf).item()) and y.isnan().all()  # inf / (inf + eps)
+    y = torch.tensor([math.inf, 1.0], device=DEV)
+    ops.clip_global_norm_([y], 1.0)  # 1 / inf = 0
+    assert y[0].isnan() and y[1] == 0.0
