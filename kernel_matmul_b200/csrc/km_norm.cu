@@ -155,17 +155,17 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_squares_kernel(const __grid
 }
 
 template <typename T>
-__device__ __forceinline__ void scale_chunk(const NormChunk &c, float f) {
+__device__ __forceinline__ void scale_chunk(const NormChunk &c, float f, float power) {
     constexpr int VEC = 16 / sizeof(T);
     T *p = reinterpret_cast<T *>(c.data);
     const int lead = (int)min(c.elements, (int64_t)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
     const int words = (int)((c.elements - lead) / VEC), tail = (int)(c.elements - lead) - words * VEC;
     uint4 *w = reinterpret_cast<uint4 *>(p + lead);
-    const auto scaled = [f](uint4 v) {
+    const auto scaled = [f, power](uint4 v) {
         T x[VEC];
         memcpy(x, &v, 16);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) x[i] = from_float<T>(as_float(x[i]) * f);
+        for (int i = 0; i < VEC; i++) x[i] = from_float<T>(as_float(x[i]) * f * power);
         memcpy(&v, x, 16);
         return v;
     };
@@ -178,10 +178,10 @@ __device__ __forceinline__ void scale_chunk(const NormChunk &c, float f) {
         for (int j = 0; j < 4; j++) w[i + j * NORM_THREADS] = scaled(v[j]);
     }
     for (; i < words; i += NORM_THREADS) w[i] = scaled(w[i]);
-    if ((int)threadIdx.x < lead) p[threadIdx.x] = from_float<T>(as_float(p[threadIdx.x]) * f);
+    if ((int)threadIdx.x < lead) p[threadIdx.x] = from_float<T>(as_float(p[threadIdx.x]) * f * power);
     if ((int)threadIdx.x < tail) {
         T *q = p + lead + words * VEC + threadIdx.x;
-        *q = from_float<T>(as_float(*q) * f);
+        *q = from_float<T>(as_float(*q) * f * power);
     }
 }
 
@@ -199,15 +199,16 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_finish_kernel(const __grid_
     if (!scale) return;
     const double factor = max_norm / (n + eps);
     if (factor >= 1.0) return;
-    const float f = (float)factor;
+    // (a factor near the smallest fp32 values or below them, as for gradients of 1e38, in two)
+    const float power = factor < 1e-30 ? 0x1p-100f : 1.0f, f = (float)(factor / (double)power);
     for (int64_t chunk = t.chunks - 1 - (int64_t)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
         const NormChunk c = norm_chunk(t, chunk);
         if (c.type == KM_TYPE_F32)
-            scale_chunk<float>(c, f);
+            scale_chunk<float>(c, f, power);
         else if (c.type == KM_TYPE_BF16)
-            scale_chunk<__nv_bfloat16>(c, f);
+            scale_chunk<__nv_bfloat16>(c, f, power);
         else
-            scale_chunk<__half>(c, f);
+            scale_chunk<__half>(c, f, power);
     }
 }
 

@@ -156,3 +156,16 @@ def test_an_infinite_bound_gives_what_the_formula_gives():
     y = torch.tensor([math.inf, 1.0], device=DEV)
     ops.clip_global_norm_([y], 1.0)  # 1 / inf = 0
     assert y[0].isnan() and y[1] == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_factors_below_the_range_of_fp32(dtype):
+    x = (torch.randn(100_003, device=DEV) * 1e37).to(dtype)
+    exact, norm = x.double(), x.double().norm().item()
+    for bound in (1e3, 1.0, 1e-3):
+        y = x.clone()
+        ops.clip_global_norm_([y], bound, eps=0.0)
+        want = exact * (bound / norm)
+        assert bound / norm < 1e-36
+        # the norm, the factor, two products and the result's rounding
+        assert ((y.double() - want).abs() <= want.abs() * (70 * 2.0**-24 + torch.finfo(dtype).eps / 2) + 2.0**-149).all()
