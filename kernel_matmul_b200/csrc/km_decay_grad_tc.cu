@@ -20,7 +20,14 @@ namespace km {
 namespace {
 
 constexpr int ARITH = 512, GRAD_THREADS = ARITH + 32;  // threads of arithmetic: four per lane of tensor memory; a warp of loads and products
-constexpr float PART = 1.0f / 128.0f;  // K' and Q' are weighted with 128ths of their distances: at most one, as fp16 needs it
+// Powers of two by which K' and Q' are scaled so that their weights, d e^{g (d - steps)} for distances d of `steps` to 127, are at most one
+// and the largest, at d = -1 / g or 1, above a half, as fp16 needs it.  (Q' has steps = 0; K', whose decays are relative to the
+// chunk's last token, that token's distance from where the chunk's state is taken: 1, or 0 at the end of a sequence.)  A slow decay's is 1/128.
+constexpr float SLOW = 1.0f / 128.0f;
+__device__ __forceinline__ float weight_scale(float g2, int steps) {
+    const float d = g2 < -0.0114f ? fmaxf(1.0f / (-0.69314718f * g2), 1.0f) : 127.0f;
+    return exp2f(-fminf(fmaxf(ceilf(log2f(d) + g2 * (d - (float)steps)), -100.0f), 7.0f));
+}
 constexpr uint32_t COL_S = 0, COL_G = 128, COL_U = 256, COL_U1 = 384;  // X' over S, X over G
 
 struct GradMaps {
@@ -91,6 +98,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, chunks = (s.count + TC - 1) / TC;
     const float g2 = log2_decay(a.log_decay[h]);
     const bool grows = HALF && g2 > 0.0f;
+    const float query_part = HALF && !grows ? weight_scale(g2, 0) : SLOW;
     if (tid == 0) {
         mbar_init(&ctl.full, 33), mbar_init(&ctl.sg_full, 1), mbar_init(&ctl.done, 1), mbar_init(&ctl.drain, 1);
         mbar_init(&ctl.ready, ARITH), mbar_init(&ctl.read, ARITH), mbar_init(&ctl.meet, ARITH);
@@ -298,19 +306,20 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
             tc_fence_before();  // (S and G have been read before X goes over them)
             ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
             if (!ok) break;
-            parts(L::K, [&](int t) { return before_last(t) * ((float)max(e - t, 0) * PART); });
+            const float key_part = HALF && !grows ? weight_scale(g2, e - last) : SLOW;
+            parts(L::K, [&](int t) { return before_last(t) * ((float)max(e - t, 0) * key_part); });
             ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
             if (!ok) break;
             if (!STATE_ONLY) {
                 parts(L::Q, behind_first);
                 ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
                 if (!ok) break;
-                parts(L::Q, [&](int t) { return behind_first(t) * ((float)t * PART); });
+                parts(L::Q, [&](int t) { return behind_first(t) * ((float)t * query_part); });
                 ok = mbar_wait_warp(&ctl.done, phase++ & 1, a.wait_polls);
                 if (!ok) break;
             }
             tc_fence_after();
-            const f32x2 carry = splat2(exp2f(g2 * (float)e)), steps = splat2((float)e), whole = splat2(1.0f / PART);
+            const f32x2 carry = splat2(exp2f(g2 * (float)e)), steps = splat2((float)e), whole = splat2(1.0f / key_part);
             const float step = exp2f(g2 * (float)(grows ? e : e - last));
             const f32x2 beyond = splat2(HALF ? step / up(0) : step);
             const f32x2 back = splat2(HALF && !STATE_ONLY ? (grows ? exp2f(g2 * (float)last) : 1.0f) / up(1) : 1.0f);  // of X and X'
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 1) decay_grad_tc_kernel(const __
                     f32x2 &zz = z[c / 2 + j], &mm = m[c / 2 + j];
                     const auto pair = [](const uint32_t &p, const uint32_t &q) { return pack2(__uint_as_float(p), __uint_as_float(q)); };
                     if (!STATE_ONLY && state_row) {  // (VB = 1: the other lanes repeat these)
-                        const f32x2 p = pair(x[2 * j], x[2 * j + 1]), p1 = mul2(whole, pair(x1[2 * j], x1[2 * j + 1]));
+                        const f32x2 p = pair(x[2 * j], x[2 * j + 1]), p1 = mul2(splat2(1.0f / query_part), pair(x1[2 * j], x1[2 * j + 1]));
                         sum = fma2(HALF ? mul2(back, p) : p, mm, sum);
                         sum = fma2(HALF ? mul2(back, p1) : p1, zz, sum);
                     }

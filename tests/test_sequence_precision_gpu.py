@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from sequence_reference import attention_with_scales, half_step
+from sequence_reference import attention, attention_with_scales, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,26 @@ def test_results_of_many_chunks_are_rounded_twice(dtype, path):
     e = evaluate(dtype, path, 1100, 8, 8, 64, 64, slopes(8))
     assert max(e["o"], e["dq"], e["dk"], e["dv"]) <= 0.65 * half_step(dtype), e
     assert not math.isnan(sum(e.values()))
+
+
+@pytest.mark.parametrize("dtype, path", [*FORMS, (torch.float32, "fma")], ids=str)
+def test_gradients_of_fast_decays(dtype, path):
+    """A decay of e^g leaves its gradient terms of e^g and smaller: each head's is held against sqrt(sum_i (go_i d o_i / d g)^2), what a sum
+    of its terms' random signs is in the mean (the last state and its gradient among them).  A term goes through fewer than 64 roundings to
+    24 bits or more; and the exponent of a decay, g log2(e) d, is rounded three times (log2(e), both products), which makes the decay
+    wrong by 3 |g| d 2^-24 of itself, where d = 1 for all terms that count."""
+    decays = -torch.tensor([1.0, 4.0, 8.0, 12.0, 16.0, 24.0, 40.0, 60.0], device=DEV)
+    draw = lambda d: torch.randn(2, 300, 8, d, device=DEV).to(dtype)  # noqa: E731
+    q, k, v, go = draw(64), draw(64), draw(40), draw(40)
+    gs = torch.randn(2, 8, 64, 40, device=DEV)
+    zero = torch.zeros_like(gs, dtype=torch.float64)
+    rest = lambda x: attention(q.double(), k.double(), v.double(), x, 64**-0.5, zero, None)  # noqa: E731
+    slope, state_slope = torch.func.jvp(rest, (decays.double(),), (torch.ones(8, device=DEV, dtype=torch.float64),))[1]
+    terms = (go.double() * slope).transpose(1, 2).flatten(2), (gs.double() * state_slope).flatten(2)  # (batch, heads, terms)
+    for used in ((0,), (1,), (0, 1)):
+        g = decays.clone().requires_grad_()
+        results = ops.decay_attention(q, k, v, g, return_state=True, path=path)
+        (got,) = torch.autograd.grad([results[i] for i in used], g, [(go, gs)[i] for i in used])
+        x = torch.cat([terms[i] for i in used], -1)
+        error = (got.double() - x.sum((0, 2))).abs() / x.square().sum((0, 2)).sqrt()
+        assert (error <= (64 + 3 * decays.abs()) * 2.0**-24).all(), error
