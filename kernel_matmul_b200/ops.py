@@ -422,8 +422,10 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *, scale
     have no gradient).  States then are ``(sequences, heads, dk, dv)``.  The values are read on the device and clamped to the rows there are.
 
     Differentiable once in ``q``, ``k``, ``v``, ``log_decay`` and ``initial_state``.  ``path``: ``"fma"``, ``"tc"`` (tensor
-    cores, 16-bit operands) or ``"auto"``.  A value that is not finite spoils its sequence's results from up to 127 tokens before
-    it on (the block in which it is multiplied), and no other sequence's or head's."""
+    cores, 16-bit operands) or ``"auto"`` (``"tc"`` for those).  On the tensor cores the product of ``q`` with the state takes a copy of it in the
+    operands' type, rounded once; ``"fma"`` keeps everything but the result in 32 bits.  A value that is not finite spoils its
+    sequence's results from up to 127 tokens before it on (the block in which it is multiplied), gradients up to 127 tokens behind it too, and no other
+    sequence's or head's; rows of no sequence may hold anything."""
     _is_cuda(q, k, v, log_decay)
     if path not in _DECAY_PATHS:
         raise ValueError(f"unknown path {path!r}")
