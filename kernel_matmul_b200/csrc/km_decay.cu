@@ -732,7 +732,7 @@ extern "C" int km_decay_attention(const km_decay_problem *problem, const km_view
     const size_t need = km_decay_attention_workspace_bytes(problem);
     KM_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KM_ERR_WORKSPACE,
                "km_decay_attention: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    KM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_decay_attention: workspace must be 16-byte aligned");
+    KM_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_decay_attention: workspace must be 16-byte aligned");
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.out = make_operand(out);
     a.state_out = make_operand(state_out);
@@ -817,7 +817,7 @@ extern "C" int km_decay_gradient(const km_decay_problem *problem, const km_view 
     const size_t need = km_decay_gradient_workspace_bytes(problem);
     KM_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KM_ERR_WORKSPACE,
                "km_decay_gradient: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    KM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_decay_gradient: workspace must be 16-byte aligned");
+    KM_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, KM_ERR_WORKSPACE, "km_decay_gradient: workspace must be 16-byte aligned");
     DecayArgs a = make_args(p, q, k, v, log_decay, starts, state_in);
     a.scale_in = 1.0f, a.scale_out = p.scale;
     const Operand d = make_operand(dout), ds = make_operand(dstate);
